@@ -1,0 +1,441 @@
+// MXFP4 (e2m1 data, two codes a byte, one power-of-two e8m0 scale per 32 elements) for sm_100a: quantisers, the expansion
+// of codes into values and the block-scaled product (tcgen05.mma kind::mxf4.block_scale).
+//
+// Scale of a group with largest magnitude amax = f 2^k (1 <= f < 2): the smallest power of two s with amax / s <= 6, that is
+// 2^(k-2) for f <= 1.5 and 2^(k-1) otherwise, stored as the byte log2(s) + 127, not below 0 (an all-zero group: 0). A group
+// that holds a NaN or an infinity gets the byte 255, the format's NaN, so that the products it enters are NaN.
+// q = e2m1(x / s), rounded to nearest with ties to even; the quotient is exact. The code of an even column is the low nibble.
+//
+// Scale tensors are in the tensor core's block layout (128 rows x 4 groups = 512 bytes, the byte of (row r, group g) at
+// (r % 32) * 16 + (r / 32) * 4 + g), as for MXFP8; padding rows and groups hold 127.
+#include "common.cuh"
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+namespace {
+using namespace fsb;
+
+// Biased exponent from the bits of amax (not negative). 0x7f800000 and above: an infinity or a NaN.
+__device__ __forceinline__ uint32_t mx4_exponent(uint32_t bits) {
+  if (bits >= 0x7f800000u) return 255u;
+  const int e = static_cast<int>(bits >> 23) - 2 + ((bits & 0x7fffffu) > 0x400000u ? 1 : 0);
+  return e < 0 ? 0u : static_cast<uint32_t>(e);
+}
+__device__ __forceinline__ float mx4_inv(uint32_t e) {   // 2^(127 - e) for e <= 253; 0 for the NaN byte (all codes 0)
+  return e == 255u ? 0.f : __uint_as_float((254u - e) << 23);
+}
+__device__ __forceinline__ float mx4_scale(uint32_t e) {   // 2^(e - 127); the NaN byte gives a NaN
+  return e == 0u ? __uint_as_float(0x00400000u) : e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(e << 23);
+}
+__device__ __forceinline__ long long blocked_offset(long long r, int g, int n_gb) {
+  return ((r >> 7) * n_gb + (g >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (g & 3);
+}
+// The magnitudes' bits order like the magnitudes, with infinities and NaN on top, so the maximum is taken on integers.
+__device__ __forceinline__ uint32_t amax8_bits(const uint4& raw, uint32_t m) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m = max(m, max(w[j] << 16 & 0x7fff0000u, w[j] & 0x7fff0000u));
+  return m;
+}
+// Eight bf16 as eight codes. x * inv is exact or rounds far below the smallest code's half step. With inv == 0 (the NaN
+// byte) infinities and NaN would give NaN, for which the conversion has no code: the codes are 0.
+__device__ __forceinline__ uint32_t quant8_fp4(const uint4& raw, float inv) {
+  if (inv == 0.f) return 0u;
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+  uint32_t o = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __bfloat1622float2(h[j]);
+    o |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(f.x * inv, f.y * inv), __NV_E2M1, cudaRoundNearest)) << (8 * j);
+  }
+  return o;
+}
+__device__ __forceinline__ uint4 load8_any(const __nv_bfloat16* p, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(p);
+  const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+  return make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
+                    h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
+}
+
+// ------------------------------------------------------------------ activation quantiser (1x32 groups)
+// Four threads per group, 8 columns each. Rows past T and groups past K / 32 get the scale byte 127.
+__global__ void __launch_bounds__(256)
+mx4_quant_act_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scales, long long T,
+                     int K, long long ldx, int n_gb, int vec) {
+  const int units = n_gb * 16;                        // threads of a padded row
+  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  const long long row = i / units;
+  const int u = static_cast<int>(i - row * units);
+  if (row >= (T + 127) / 128 * 128) return;           // the four threads of a group leave together
+  const bool live = row < T && u * 8 < K;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (live) v = load8_any(x + row * ldx + u * 8, vec);
+  uint32_t m = amax8_bits(v, 0u);
+  const unsigned group = 0xfu << (threadIdx.x & 28);
+  m = max(m, __shfl_xor_sync(group, m, 2));
+  m = max(m, __shfl_xor_sync(group, m, 1));
+  const uint32_t e = mx4_exponent(m);
+  if ((u & 3) == 0) scales[blocked_offset(row, u >> 2, n_gb)] = live ? static_cast<uint8_t>(e) : 127;
+  if (live) *reinterpret_cast<uint32_t*>(q + row * (K / 2) + u * 4) = quant8_fp4(v, mx4_inv(e));
+}
+
+// ------------------------------------------------------------------ weight quantiser (32x32 tiles)
+// A warp per tile: lane l holds 8 columns of rows l/4, l/4 + 8, l/4 + 16, l/4 + 24. One tile exponent serves the forward
+// product (groups along the columns) and the input gradient (groups along the rows). Besides the tile exponents it can write
+// the blocked scales of both operands: tiles past the edges, up to whole 128 x 128 blocks, write the padding.
+__global__ void __launch_bounds__(128)
+mx4_quant_weight_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __restrict__ q, uint8_t* __restrict__ tile_exp,
+                        uint8_t* __restrict__ fwd, uint8_t* __restrict__ dgrad, int rows, int cols, long long ldw, int vec) {
+  const int tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int exp_rows = (rows + 31) / 32, exp_cols = cols / 32, rt = blockIdx.y;
+  const bool inside = rt < exp_rows && tile < exp_cols;
+  uint32_t e = 127;
+  if (inside) {
+    const int r0 = rt * 32 + (lane >> 2), c0 = tile * 32 + (lane & 3) * 8;
+    uint4 v[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + 8 * i;
+      v[i] = r < rows ? load8_any(w + r * ldw + c0, vec) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = amax8_bits(v[i], m);
+    m = __reduce_max_sync(0xffffffffu, m);
+    e = mx4_exponent(m);
+    if (lane == 0) tile_exp[static_cast<long long>(rt) * exp_cols + tile] = static_cast<uint8_t>(e);
+    const float inv = mx4_inv(e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + 8 * i;
+      if (r < rows) *reinterpret_cast<uint32_t*>(q + static_cast<long long>(r) * (cols / 2) + c0 / 2) = quant8_fp4(v[i], inv);
+    }
+  }
+  const int col_blocks = (cols + 127) / 128, row_blocks = (rows + 127) / 128;
+  if (fwd != nullptr) {
+    const long long r = static_cast<long long>(rt) * 32 + lane;
+    fwd[blocked_offset(r, tile, col_blocks)] = static_cast<uint8_t>(r < rows ? e : 127);
+  }
+  if (dgrad != nullptr) dgrad[blocked_offset(static_cast<long long>(tile) * 32 + lane, rt, row_blocks)] = static_cast<uint8_t>(e);
+}
+
+// ------------------------------------------------------------------ expansion
+// Codes as the values they stand for: e4m3 without the scales (kind 0, every e2m1 value is one of e4m3), bf16 (1) or fp32 (2)
+// with them. e2m1 values times powers of two are exact in all three, but for what underflows. Eight codes a thread.
+__global__ void __launch_bounds__(256)
+mx4_expand_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, void* __restrict__ out, long long T, int K,
+                  long long ldq, int n_gb, int kind) {
+  const int units = K / 8;
+  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  const long long row = i / units;
+  if (row >= T) return;
+  const int u = static_cast<int>(i - row * units);
+  const uint32_t c = *reinterpret_cast<const uint32_t*>(q + row * ldq + u * 4);
+  const float s = kind == 0 ? 1.f : mx4_scale(scales[blocked_offset(row, u >> 2, n_gb)]);
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t code = c >> (4 * j), mag = code & 7u;
+    // magnitudes 0, .5, then (1 + mantissa / 2) 2^(exponent - 1)
+    const float a = mag < 2 ? 0.5f * mag : __uint_as_float((126u + (mag >> 1)) << 23 | (mag & 1u) << 22);
+    f[j] = (code & 8u ? -a : a) * s;
+  }
+  const long long at = row * K + u * 8;
+  if (kind == 2) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+    d[0] = make_float4(f[0], f[1], f[2], f[3]);
+    d[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else if (kind == 1) {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at) =
+        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  } else {
+    uint2 o;
+    uint16_t* h = reinterpret_cast<uint16_t*>(&o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * j], f[2 * j + 1]), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(out) + at) = o;
+  }
+}
+
+// ------------------------------------------------------------------ block-scaled product
+// out[t, n] = sum_k a[t, k] b[n, k]. The weight b is the tensor core's M operand (128 rows a tile), the rows t its N operand,
+// so that a tile of few rows costs few columns. A stage is 256 deep (128 bytes a row, the swizzle's width): four 64-deep MMAs,
+// each with two scale bytes a row. The scales travel as whole blocks (two per 128 rows and stage) and are copied to TMEM right
+// before the MMAs. Codes past K read as zeros; so do scale blocks past the last one.
+constexpr int BM = 128, BK = 256, KB = BK / 2;      // KB: bytes of a row in a stage
+constexpr int SF_BYTES = 1024;                      // two scale blocks
+constexpr int NUM_THREADS = 192;                    // warp 0 TMA, warp 1 MMA, warps 2..5 epilogue
+
+template <int BN>
+struct Tile {
+  static constexpr int A_STAGE = BM * KB, B_STAGE = BN * KB;
+  static constexpr int STAGE_BYTES = A_STAGE + B_STAGE + 2 * SF_BYTES;   // a multiple of 1 KB for BN >= 16 in steps of 8
+  static constexpr int STAGES = 4;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+  static constexpr int SF_COL0 = BN < 32 ? 32 : BN;                      // first scale column
+  static constexpr int TMEM_COLS = BN <= 64 ? 128 : 256;                 // accumulator + two sets of 8 + 8 scale columns
+};
+
+struct Args {
+  int M, N, K;
+  void* d;
+  long long ldd;
+  int d_fp32;
+  int* status;
+};
+
+__device__ __forceinline__ void tmem_cp_32x128b_x4(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// Unswizzled K-major descriptor: 8-row groups of 16-byte rows are 128 bytes apart.
+__device__ __forceinline__ uint64_t make_sf_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(128 >> 4) << 32;   // SBO
+  d |= 1ull << 46;
+  return d;
+}
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tsfa,
+                                          uint32_t tsfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tsfa), "r"(tsfb)
+      : "memory");
+}
+// e2m1 x e2m1 (format 1 of this kind), e8m0 scales, both operands K-major; sf_id: first of the scale word's bytes used (0, 2)
+__device__ __forceinline__ constexpr uint32_t make_idesc_mx4(uint32_t m, uint32_t n, uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (sf_id << 29);
+}
+
+template <int BN>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                  const __grid_constant__ CUtensorMap map_sfw, const __grid_constant__ CUtensorMap map_sfx, const Args args) {
+  using S = Tile<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE_BYTES);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + S::STAGES;
+  uint64_t* tmem_full = bars + 2 * S::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::STAGES + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tw = blockIdx.x, tx = blockIdx.y;
+  const int num_kb = (args.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(tmem_full, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&map_w);
+      tma_prefetch_desc(&map_x);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        const int s = kb % S::STAGES;
+        if (!mbar_wait(&empty_bar[s], ((kb / S::STAGES) & 1) ^ 1, abort_flag)) {
+          atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_EMPTY);
+          *abort_flag = 1;
+          break;
+        }
+        uint8_t* sa = smem + s * S::STAGE_BYTES;
+        uint8_t* sb = sa + S::A_STAGE;
+        uint8_t* ssf = sb + S::B_STAGE;
+        mbar_expect_tx(&full_bar[s], S::STAGE_BYTES);
+        tma_load_2d(sa, &map_w, &full_bar[s], kb * KB, tw * BM);
+        tma_load_2d(sb, &map_x, &full_bar[s], kb * KB, tx * BN);
+        tma_load_2d(ssf, &map_sfw, &full_bar[s], kb * 256, tw);                        // 256 words: two blocks
+        tma_load_2d(ssf + SF_BYTES, &map_sfx, &full_bar[s], kb * 256, tx * BN / 128);
+      }
+    }
+  } else if (warp == 1) {
+    // The whole warp walks the loop; one elected lane issues the tcgen05 instructions.
+    bool ok = true;
+    for (int kb = 0; kb < num_kb; ++kb) {
+      const int s = kb % S::STAGES;
+      if (!mbar_wait(&full_bar[s], (kb / S::STAGES) & 1, abort_flag)) {
+        if (lane == 0) {
+          atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_FULL);
+          *abort_flag = 1;
+        }
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sa = smem_u32(smem + s * S::STAGE_BYTES);
+      const uint64_t da = make_smem_desc_sw128(sa, 16, 1024);
+      const uint64_t db = make_smem_desc_sw128(sa + S::A_STAGE, 16, 1024);
+      const uint32_t ssf = sa + S::A_STAGE + S::B_STAGE;
+      const uint32_t tsf = tmem_base + S::SF_COL0 + (kb & 1) * 16;   // 2 x 4 columns of weight scales, 2 x 4 of row scales
+      if (elect_one()) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tmem_cp_32x128b_x4(tsf + 4 * h, make_sf_desc(ssf + 512 * h));
+          tmem_cp_32x128b_x4(tsf + 8 + 4 * h, make_sf_desc(ssf + SF_BYTES + 512 * h));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_mxf4(tmem_base, da + 2 * k, db + 2 * k, make_idesc_mx4(BM, BN, (k & 1) * 2), tsf + 4 * (k >> 1),
+                    tsf + 8 + 4 * (k >> 1), (kb | k) != 0);
+        umma_commit(&empty_bar[s]);
+      }
+      __syncwarp();
+    }
+    if (ok) {
+      if (elect_one()) umma_commit(tmem_full);
+      __syncwarp();
+    }
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int n = tw * BM + quarter * 32 + lane;
+    if (!mbar_wait_warp(tmem_full, 0, abort_flag)) {
+      if (lane == 0) {
+        atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_TMEM_FULL);
+        *abort_flag = 1;
+      }
+    } else {
+      tc_fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld_32x16(t_row + c0, v);
+        tmem_ld_wait();
+        if (n >= args.N) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const long long t = static_cast<long long>(tx) * BN + c0 + i;
+          if (t >= args.M) break;
+          if (args.d_fp32) static_cast<float*>(args.d)[t * args.ldd + n] = __uint_as_float(v[i]);
+          else static_cast<__nv_bfloat16*>(args.d)[t * args.ldd + n] = __float2bfloat16(__uint_as_float(v[i]));
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (*abort_flag) {
+      const unsigned long long t0 = clock64();
+      while (clock64() - t0 < 2000000ull) {
+      }
+    }
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::TMEM_COLS);
+  }
+}
+
+inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH; }
+
+// codes [rows, K] as bytes, boxes of box_rows rows x 128 bytes
+int codes_map(CUtensorMap* map, const void* q, long long rows, int K, long long ld, int box_rows) {
+  return fsb_make_tmap_2d(map, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, K / 2, ld, box_rows, KB);
+}
+// blocked scales: one row of n_gb * 128 words per 128 operand rows, boxes of box_rows rows x two blocks
+int scales_map(CUtensorMap* map, const void* sf, long long rows, int K, int box_rows) {
+  const uint64_t words = static_cast<uint64_t>((K + 127) / 128) * 128;
+  return fsb_make_tmap_2d_plain(map, sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (rows + 127) / 128, words, words, box_rows, 256);
+}
+
+template <int BN>
+int launch(const void* aq, const void* sfa, const void* bq, const void* sfb, const Args& a, long long lda, long long ldb,
+           cudaStream_t stream) {
+  static bool raised[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return FSB_ERR_BAD_ARG;
+  if (!raised[dev]) {
+    if (cudaFuncSetAttribute(gemm_mxfp4_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<BN>::SMEM) != cudaSuccess)
+      return FSB_ERR_LAUNCH;
+    raised[dev] = true;
+  }
+  CUtensorMap map_w, map_x, map_sfw, map_sfx;
+  int rc = codes_map(&map_w, bq, a.N, a.K, ldb, BM);
+  if (rc == FSB_OK) rc = codes_map(&map_x, aq, a.M, a.K, lda, BN);
+  if (rc == FSB_OK) rc = scales_map(&map_sfw, sfb, a.N, a.K, 1);
+  if (rc == FSB_OK) rc = scales_map(&map_sfx, sfa, a.M, a.K, 1);
+  if (rc != FSB_OK) return rc;
+  const dim3 grid((a.N + BM - 1) / BM, (a.M + BN - 1) / BN);
+  if (grid.y > 65535) return FSB_ERR_TOO_LARGE;
+  gemm_mxfp4_kernel<BN><<<grid, NUM_THREADS, Tile<BN>::SMEM, stream>>>(map_w, map_x, map_sfw, map_sfx, a);
+  return ok();
+}
+}  // namespace
+
+// x: bf16 [T, K], K % 32 == 0, row stride ldx; q: [T, K / 2] bytes; scales: pad128(T) * pad4(K / 32) bytes, all written.
+FSB_API int fsb_mx4_quant_act(const void* x, void* q, void* scales, long long T, int K, long long ldx, cudaStream_t stream) {
+  if (K <= 0 || K % 32 != 0 || T < 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0) return FSB_ERR_BAD_ARG;
+  if (T == 0) return FSB_OK;
+  const int n_gb = (K + 127) / 128;
+  const long long blocks = ((T + 127) / 128 * 128 * (n_gb * 16) + 255) / 256;
+  if (blocks > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
+  const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx % 8 == 0;
+  mx4_quant_act_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+      static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales), T, K, ldx, n_gb, vec);
+  return ok();
+}
+
+// w: bf16 [rows, cols], cols % 32 == 0; q: [rows, cols / 2] bytes; tile_exp: [ceil(rows / 32), cols / 32] bytes. fwd / dgrad
+// (each may be null): blocked scales of the operands [rows, cols] and [cols, rows], padding included.
+FSB_API int fsb_mx4_quant_weight(const void* w, void* q, void* tile_exp, void* fwd, void* dgrad, int rows, int cols, long long ldw,
+                                 cudaStream_t stream) {
+  if (rows < 0 || cols <= 0 || cols % 32 != 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0) return FSB_ERR_BAD_ARG;
+  if (rows == 0) return FSB_OK;
+  const dim3 grid((cols + 127) / 128, (rows + 127) / 128 * 4);
+  if (grid.y > 65535) return FSB_ERR_TOO_LARGE;
+  const int vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && ldw % 8 == 0;
+  mx4_quant_weight_kernel<<<grid, 128, 0, stream>>>(static_cast<const __nv_bfloat16*>(w), static_cast<uint8_t*>(q),
+                                                    static_cast<uint8_t*>(tile_exp), static_cast<uint8_t*>(fwd),
+                                                    static_cast<uint8_t*>(dgrad), rows, cols, ldw, vec);
+  return ok();
+}
+
+// q: [T, K / 2] codes with row stride ldq bytes; scales: blocked (not read for kind 0); out: [T, K] contiguous, e4m3 without
+// scales (kind 0), bf16 (1) or fp32 (2).
+FSB_API int fsb_mx4_expand(const void* q, const void* scales, void* out, long long T, int K, long long ldq, int kind,
+                           cudaStream_t stream) {
+  if (K <= 0 || K % 32 != 0 || T < 0 || ldq % 4 != 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0 || kind < 0 || kind > 2)
+    return FSB_ERR_BAD_ARG;
+  if (T == 0) return FSB_OK;
+  const long long blocks = (T * (K / 8) + 255) / 256;
+  if (blocks > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
+  mx4_expand_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const uint8_t*>(q),
+                                                                      static_cast<const uint8_t*>(scales), out, T, K, ldq,
+                                                                      (K + 127) / 128, kind);
+  return ok();
+}
+
+// d[M, N] = A B^T for codes aq [M, K / 2] and bq [N, K / 2] (row strides lda, ldb bytes, multiples of 16) with blocked scales
+// sfa, sfb; K % 32 == 0.
+FSB_API int fsb_gemm_mxfp4(const void* aq, const void* sfa, const void* bq, const void* sfb, void* d, int M, int N, int K,
+                           long long lda, long long ldb, long long ldd, int d_fp32, int* status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || lda % 16 != 0 || ldb % 16 != 0) return FSB_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(sfa) | reinterpret_cast<uintptr_t>(sfb) | reinterpret_cast<uintptr_t>(aq) |
+       reinterpret_cast<uintptr_t>(bq)) & 15)
+    return FSB_ERR_BAD_ARG;
+  Args a;
+  a.M = M; a.N = N; a.K = K;
+  a.d = d; a.ldd = ldd; a.d_fp32 = d_fp32; a.status = status;
+  if (M <= 16) return launch<16>(aq, sfa, bq, sfb, a, lda, ldb, stream);
+  if (M <= 32) return launch<32>(aq, sfa, bq, sfb, a, lda, ldb, stream);
+  if (M <= 64) return launch<64>(aq, sfa, bq, sfb, a, lda, ldb, stream);
+  return launch<128>(aq, sfa, bq, sfb, a, lda, ldb, stream);
+}

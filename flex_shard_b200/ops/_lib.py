@@ -7,6 +7,7 @@ False and callers use their CPU reference paths.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -123,6 +124,15 @@ def stream_ptr(device=None) -> int:
     5 us a call; a small training step makes 70 to 120 launches)."""
     index = device.index if isinstance(device, torch.device) else device
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+_same_device = contextlib.nullcontext()
+
+
+def device_of(tensor):
+    """Context in which the device of ``tensor`` is the current one (a launch onto a stream needs its device current)."""
+    index = tensor.device.index
+    return _same_device if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def plain(*tensors) -> bool:

@@ -154,10 +154,15 @@ class _Linear(torch.autograd.Function):
 
 def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """``x @ weight.T``. A weight handed out by a quantised-gather placement (FP8 128x128 blocks or
-    MXFP8) runs the matching block-scaled products; its gradient still goes to the logical parameter."""
+    MXFP8) runs the matching block-scaled products; its gradient still goes to the logical parameter. A frozen MXFP4
+    weight (``BlockwiseMxfp4Weight``) runs the 4-bit product and takes no gradient."""
     if type(weight) is not torch.Tensor and type(weight) is not torch.nn.Parameter:
-        from ..quant.weight import BlockwiseFp8Weight, BlockwiseMxfp8Weight
+        from ..quant.weight import BlockwiseFp8Weight, BlockwiseMxfp4Weight, BlockwiseMxfp8Weight
 
+        if isinstance(weight, BlockwiseMxfp4Weight):
+            from .mxfp4 import mxfp4_linear
+
+            return mxfp4_linear(x, None, weight.qdata, weight.scale, weight.dgrad_scale)
         if isinstance(weight, BlockwiseMxfp8Weight):
             from .mxfp8 import mxfp8_linear
 

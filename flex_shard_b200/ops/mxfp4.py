@@ -1,0 +1,302 @@
+"""MXFP4: e2m1 data (two codes a byte) with one power-of-two (e8m0) scale per 32 elements, quantisers and the
+block-scaled tcgen05 GEMM (``kind::mxf4.block_scale``), with a linear autograd function.
+
+Contract (the "round up" scaling rule of the MXFP8 operators, for a largest magnitude of 6): the scale of a group is the
+smallest power of two ``s`` with ``amax / s <= 6``, stored as the byte ``log2(s) + 127`` (not below 0; 0 for an all-zero
+group), ``q = e2m1(x / s)`` rounded to nearest with ties to even. A group that holds a NaN or an infinity gets the byte 255
+(the format's NaN) and codes of 0: what it is multiplied into is NaN. Weights use 32x32 tiles, so that one set of tile
+exponents serves the forward product and the input-gradient product; activations use 1x32 groups.
+
+Codes are uint8 tensors ``[rows, cols / 2]``, the code of an even column in the low nibble. Scale tensors handed to the GEMM
+are in the tensor core's block layout (``ops/mxfp8.py``). Columns are a multiple of 32. CPU tensors take a PyTorch
+restatement of the same arithmetic.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import count_launch
+from .gemm import gemm
+from .mxfp8 import GROUP, MX_WGRAD, blocked_scale_numel, from_blocked, gemm_mxfp8, mx_quantize_act, mx_quantize_rows, to_blocked
+
+FP8 = torch.float8_e4m3fn
+_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+_KINDS = {FP8: 0, torch.bfloat16: 1, torch.float32: 2}
+_declared = False
+
+
+def _ensure():
+    global _declared
+    if not _declared:
+        c = ctypes
+        vp, i32, i64 = c.c_void_p, c.c_int, c.c_longlong
+        _lib.declare("fsb_mx4_quant_act", [vp, vp, vp, i64, i32, i64, vp])
+        _lib.declare("fsb_mx4_quant_weight", [vp, vp, vp, vp, vp, i32, i32, i64, vp])
+        _lib.declare("fsb_mx4_expand", [vp, vp, vp, i64, i32, i64, i32, vp])
+        _lib.declare("fsb_gemm_mxfp4", [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, vp, vp])
+        _declared = True
+
+
+def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+    """Checked bf16 ``[rows, cols]`` with dense rows."""
+    if x.dim() != 2 or x.shape[1] % GROUP or x.shape[1] == 0:
+        raise ValueError(f"{what} must be a matrix whose columns are a multiple of {GROUP}, got {tuple(x.shape)}")
+    if not x.is_floating_point():
+        raise ValueError(f"{what} must be floating point, got {x.dtype}")
+    x = x.detach()
+    return x if (x.dtype == torch.bfloat16 and x.stride(1) == 1) else x.to(torch.bfloat16).contiguous()
+
+
+def _check_operand(q: torch.Tensor, scales: torch.Tensor, what: str) -> None:
+    if q.dim() != 2 or q.dtype != torch.uint8 or q.shape[1] % (GROUP // 2) or q.shape[1] == 0:
+        raise ValueError(f"{what}: codes must be a uint8 matrix [rows, cols / 2] with cols a multiple of {GROUP}, got "
+                         f"{q.dtype}{tuple(q.shape)}")
+    need = blocked_scale_numel(q.shape[0], 2 * q.shape[1])
+    if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.numel() < need or scales.device != q.device:
+        raise ValueError(f"{what}: scales must be at least {need} contiguous uint8 bytes in block layout on the codes' device")
+
+
+# --------------------------------------------------------------------------- restatement
+def _exponent(amax: torch.Tensor) -> torch.Tensor:
+    bits = amax.float().contiguous().view(torch.int32)
+    e = ((bits >> 23) - 2 + ((bits & 0x7FFFFF) > 0x400000).int()).clamp_min(0)
+    return torch.where(bits >= 0x7F800000, torch.full_like(e, 255), e).to(torch.uint8)
+
+
+def _scale(e: torch.Tensor) -> torch.Tensor:
+    """``2^(e - 127)``, NaN for 255."""
+    b = e.to(torch.int32)
+    s = torch.where(b == 0, torch.full_like(b, 0x00400000), b << 23).view(torch.float32)
+    return torch.where(b == 255, torch.full_like(s, float("nan")), s)
+
+
+def _encode(t: torch.Tensor, e: torch.Tensor) -> torch.Tensor:
+    """Codes of fp32 values whose scale bytes ``e`` broadcast against them."""
+    v = t * _scale((254 - e.to(torch.int32)).clamp_min(0).to(torch.uint8))
+    v = torch.where(e == 255, torch.zeros_like(v), v)
+    a = v.abs()
+    # between the magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6; a midpoint goes to the even code
+    code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
+    return code | torch.signbit(v).to(torch.uint8) << 3
+
+
+def _pack(codes: torch.Tensor) -> torch.Tensor:
+    return codes[:, 0::2] | codes[:, 1::2] << 4
+
+
+def _unpack(q: torch.Tensor) -> torch.Tensor:
+    return torch.stack([q & 15, q >> 4], -1).reshape(q.shape[0], 2 * q.shape[1])
+
+
+def mx4_quantize_act_ref(x: torch.Tensor):
+    T, K = x.shape
+    t = x.to(torch.bfloat16).float().reshape(T, K // GROUP, GROUP)
+    e = _exponent(t.abs().amax(-1))
+    return _pack(_encode(t, e[..., None]).view(T, K)), to_blocked(e)
+
+
+def mx4_quantize_weight_ref(w: torch.Tensor):
+    rows, cols = w.shape
+    pad = torch.zeros(-(-rows // GROUP) * GROUP, cols, dtype=torch.float32, device=w.device)
+    pad[:rows] = w.to(torch.bfloat16).float()
+    t = pad.view(-1, GROUP, cols // GROUP, GROUP)
+    e = _exponent(t.abs().amax(dim=(1, 3)))
+    return _pack(_encode(t, e[:, None, :, None]).view(-1, cols)[:rows]).contiguous(), e
+
+
+# --------------------------------------------------------------------------- quantisers
+def mx4_quantize_act(x: torch.Tensor):
+    """bf16 ``[T, K]`` -> (codes ``[T, K / 2]``, blocked uint8 scales), groups of 32 along the row. Other floating types
+    are rounded to bf16 first."""
+    x = _matrix(x, "the input")
+    if not x.is_cuda:
+        return mx4_quantize_act_ref(x)
+    _ensure()
+    T, K = x.shape
+    q = torch.empty(T, K // 2, dtype=torch.uint8, device=x.device)
+    s = torch.empty(blocked_scale_numel(T, K), dtype=torch.uint8, device=x.device)
+    with _lib.device_of(x):
+        rc = _lib.load().fsb_mx4_quant_act(x.data_ptr(), q.data_ptr(), s.data_ptr(), T, K, x.stride(0), _lib.stream_ptr(x.device))
+    _lib.check(rc, "fsb_mx4_quant_act")
+    count_launch(int(T > 0))
+    return q, s
+
+
+def _quantize_weight(w: torch.Tensor, layouts: bool):
+    rows, cols = w.shape
+    empty = lambda *n: torch.empty(*n, dtype=torch.uint8, device=w.device)  # noqa: E731
+    q, e = empty(rows, cols // 2), empty(-(-rows // GROUP), cols // GROUP)
+    fwd = empty(blocked_scale_numel(rows, cols)) if layouts else None
+    dgrad = empty(blocked_scale_numel(cols, rows)) if layouts else None
+    with _lib.device_of(w):
+        rc = _lib.load().fsb_mx4_quant_weight(w.data_ptr(), q.data_ptr(), e.data_ptr(), fwd.data_ptr() if layouts else None,
+                                              dgrad.data_ptr() if layouts else None, rows, cols, w.stride(0),
+                                              _lib.stream_ptr(w.device))
+    _lib.check(rc, "fsb_mx4_quant_weight")
+    count_launch(int(rows > 0))
+    return q, e, fwd, dgrad
+
+
+def mx4_quantize_weight(w: torch.Tensor):
+    """bf16 ``[rows, cols]`` -> (codes ``[rows, cols / 2]``, uint8 tile exponents ``[ceil(rows / 32), cols / 32]``)."""
+    w = _matrix(w, "the weight")
+    if not w.is_cuda:
+        return mx4_quantize_weight_ref(w)
+    _ensure()
+    return _quantize_weight(w, False)[:2]
+
+
+def mx4_quantize_weight_operands(w: torch.Tensor):
+    """As ``mx4_quantize_weight`` with both operands' blocked scales from the same pass: (codes, tile exponents, scales of
+    ``[rows, cols]`` for the forward product, scales of ``[cols, rows]`` for the input-gradient product)."""
+    w = _matrix(w, "the weight")
+    if not w.is_cuda:
+        from .mxfp8 import mx_expand_scales
+
+        q, e = mx4_quantize_weight_ref(w)
+        return q, e, mx_expand_scales(e, *w.shape, False), mx_expand_scales(e, *w.shape, True)
+    _ensure()
+    return _quantize_weight(w, True)
+
+
+def _expand(q: torch.Tensor, scales, dtype: torch.dtype) -> torch.Tensor:
+    _ensure()
+    T, K = q.shape[0], 2 * q.shape[1]
+    if q.stride(1) != 1 or q.stride(0) % 4 or q.data_ptr() % 4:
+        q = q.contiguous()
+    out = torch.empty(T, K, dtype=dtype, device=q.device)
+    with _lib.device_of(q):
+        rc = _lib.load().fsb_mx4_expand(q.data_ptr(), scales.data_ptr() if scales is not None else None, out.data_ptr(), T, K,
+                                        q.stride(0), _KINDS[dtype], _lib.stream_ptr(q.device))
+    _lib.check(rc, "fsb_mx4_expand")
+    count_launch(int(T > 0))
+    return out
+
+
+def mx4_dequantize(q: torch.Tensor, blocked: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Codes ``[rows, cols / 2]`` with blocked scales whose groups run along the columns -> ``[rows, cols]`` in bf16 or fp32
+    (exact in both, but for what underflows)."""
+    _check_operand(q, blocked, "mx4_dequantize")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"mx4_dequantize gives bf16 or fp32, not {dtype}")
+    if q.is_cuda:
+        return _expand(q, blocked, dtype)
+    c = _unpack(q).long()
+    v = torch.tensor(_VALUES)[c & 7] * (1 - 2 * (c >> 3))
+    e = from_blocked(blocked, q.shape[0], c.shape[1] // GROUP)
+    return (v * _scale(e).repeat_interleave(GROUP, 1)).to(dtype)
+
+
+def mx4_to_e4m3(q: torch.Tensor) -> torch.Tensor:
+    """The codes' values, without scales, as e4m3 ``[rows, cols]``: the same operand for the 8-bit products (exact)."""
+    if q.dim() != 2 or q.dtype != torch.uint8 or q.shape[1] % (GROUP // 2) or q.shape[1] == 0:
+        raise ValueError(f"codes must be a uint8 matrix [rows, cols / 2] with cols a multiple of {GROUP}")
+    if q.is_cuda:
+        return _expand(q, None, FP8)
+    c = _unpack(q).long()
+    return (torch.tensor(_VALUES)[c & 7] * (1 - 2 * (c >> 3))).to(FP8)
+
+
+# --------------------------------------------------------------------------- GEMM
+def gemm_mxfp4(aq, sfa, bq, sfb, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``out[M, N] = (A * 2^sfa) . (B * 2^sfb)^T`` for codes ``aq [M, K / 2]`` and ``bq [N, K / 2]`` with blocked scales,
+    accumulated in fp32, rounded once (bf16) or not (fp32)."""
+    _check_operand(aq, sfa, "gemm_mxfp4: left operand")
+    _check_operand(bq, sfb, "gemm_mxfp4: right operand")
+    if aq.shape[1] != bq.shape[1] or aq.device != bq.device:
+        raise ValueError(f"gemm_mxfp4: operands {tuple(aq.shape)} and {tuple(bq.shape)} on {aq.device} and {bq.device}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"gemm_mxfp4 gives bf16 or fp32, not {out_dtype}")
+    M, N, K = aq.shape[0], bq.shape[0], 2 * aq.shape[1]
+    if not aq.is_cuda:
+        return (mx4_dequantize(aq, sfa, torch.float32) @ mx4_dequantize(bq, sfb, torch.float32).t()).to(out_dtype)
+    out = torch.empty(M, N, dtype=out_dtype, device=aq.device)
+    if M == 0 or N == 0:
+        return out
+    _ensure()
+    aq, bq = (t if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0 else t.contiguous() for t in (aq, bq))
+    sfa, sfb = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (sfa, sfb))
+    status = _lib.status_word(aq.device)
+    with _lib.device_of(aq):
+        rc = _lib.load().fsb_gemm_mxfp4(aq.data_ptr(), sfa.data_ptr(), bq.data_ptr(), sfb.data_ptr(), out.data_ptr(), M, N, K,
+                                        aq.stride(0), bq.stride(0), out.stride(0), int(out_dtype == torch.float32),
+                                        status.data_ptr(), _lib.stream_ptr(aq.device))
+    _lib.check(rc, "fsb_gemm_mxfp4")
+    count_launch()
+    return out
+
+
+def _whole_octets(t: torch.Tensor) -> torch.Tensor:
+    """Rows padded with zeros to a multiple of 8, which the bf16 product over the rows needs."""
+    return t if t.shape[0] % 8 == 0 else torch.nn.functional.pad(t, (0, 0, 0, -t.shape[0] % 8))
+
+
+class _Mxfp4Linear(torch.autograd.Function):
+    """y = x W^T in 4 bits; gradients in 8 bits with the 4-bit weights' own values (quantisation counts as the identity)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, wq, fwd_scale, dgrad_scale):
+        x2 = x.reshape(-1, x.shape[-1])
+        ctx.save_for_backward(x2, wq, dgrad_scale)
+        ctx.xshape = x.shape
+        ctx.weight = weight
+        xq, sx = mx4_quantize_act(x2)
+        return gemm_mxfp4(xq, sx, wq, fwd_scale).view(*x.shape[:-1], wq.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, wq, dgrad_scale = ctx.saved_tensors
+        weight = ctx.weight
+        N, K = wq.shape[0], x2.shape[1]
+        dy2 = dy.reshape(-1, N).contiguous()
+        T = dy2.shape[0]
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            if T == 0:
+                dx = torch.zeros(ctx.xshape, dtype=x2.dtype, device=x2.device)
+            else:
+                dyq, sdy = mx_quantize_act(dy2)
+                dx = gemm_mxfp8(dyq, sdy, mx4_to_e4m3(wq), dgrad_scale, b_t=True).view(ctx.xshape)
+        if ctx.needs_input_grad[1]:
+            main = getattr(weight, "main_grad", None)
+            gd = getattr(weight, "grad_dtype", None) or torch.bfloat16
+            gd = gd if gd in (torch.bfloat16, torch.float32) else torch.bfloat16
+            if main is not None and main.dtype in (torch.float32, torch.bfloat16):
+                if T > 0:
+                    gemm(_whole_octets(dy2), _whole_octets(x2), a_t=True, b_t=True, out=main,
+                         accumulate=bool(getattr(weight, "main_grad_written", False)))
+                    weight.main_grad_written = True
+            elif T == 0:
+                dw = torch.zeros(N, K, dtype=gd, device=x2.device)
+            elif MX_WGRAD and T % 128 == 0 and N % 128 == 0 and K % 128 == 0:
+                # contraction over the tokens: both operands in 32x1 groups, read transposed by the tensor core
+                dq, sd = mx_quantize_rows(dy2)
+                xq, sx = mx_quantize_rows(x2)
+                dw = gemm_mxfp8(dq, sd, xq, sx, a_t=True, b_t=True, out_dtype=gd)
+            else:
+                dw = gemm(_whole_octets(dy2), _whole_octets(x2), a_t=True, b_t=True, out_dtype=gd)
+        return dx, dw, None, None, None
+
+
+def mxfp4_linear(x, weight, wq, fwd_scale, dgrad_scale):
+    """``x @ W.T`` for bf16 ``x [..., K]`` (K a multiple of 32) and a weight given as MXFP4 codes ``wq [N, K / 2]`` with the
+    blocked scales of the operands ``[N, K]`` (forward) and ``[K, N]`` (input gradient; may be ``None`` where no gradient
+    of ``x`` is asked for). ``weight`` is the logical parameter that receives the weight gradient, or ``None`` for a frozen
+    weight. Gradients run on the 8-bit products and need N and K in multiples of 128 (``x``'s) and of 8 (the weight's)."""
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"mxfp4_linear takes bf16 inputs, got {x.dtype}")
+    if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != 2 * wq.shape[1]:
+        raise ValueError(f"mxfp4_linear: input {tuple(x.shape)} does not match codes {tuple(wq.shape)} ([N, K / 2])")
+    N, K = wq.shape[0], x.shape[-1]
+    if torch.is_grad_enabled():
+        if x.requires_grad:
+            if N % 128 or K % 128:
+                raise ValueError(f"the input gradient of mxfp4_linear needs dims that are multiples of 128, got {N} x {K}")
+            if dgrad_scale is None:
+                raise ValueError("the input gradient of mxfp4_linear needs the scales of the transposed weight (dgrad_scale)")
+        if weight is not None and weight.requires_grad and (N % 8 or K % 8):
+            raise ValueError(f"the weight gradient of mxfp4_linear needs dims that are multiples of 8, got {N} x {K}")
+    return _Mxfp4Linear.apply(x, weight, wq, fwd_scale, dgrad_scale)

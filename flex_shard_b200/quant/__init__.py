@@ -2,15 +2,18 @@
 from .linear import (
     FlexShardFloat8BlockwiseLinear,
     FlexShardFloat8BlockwiseStackedLinear,
+    FlexShardMxfp4BlockwiseLinear,
     FlexShardMxfp8BlockwiseLinear,
     FlexShardPrequantizedLinear,
     PrequantizedLinearGemms,
     convert_to_flex_shard_float8_blockwise_linear,
+    convert_to_flex_shard_mxfp4_blockwise_linear,
     convert_to_flex_shard_mxfp8_blockwise_linear,
     convert_to_flex_shard_prequantized_linear,
 )
 from .weight import (
     BlockwiseFp8Weight,
+    BlockwiseMxfp4Weight,
     BlockwiseMxfp8Weight,
     BlockwiseQuantWeight,
     blockwise_dequant_weight,

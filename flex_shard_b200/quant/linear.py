@@ -17,8 +17,9 @@ import torch
 import torch.nn as nn
 
 from ..ops.fp8 import fp8_linear, quantize_blockwise
+from ..ops.mxfp4 import mxfp4_linear
 from ..ops.mxfp8 import mx_expand_scales, mx_quantize_weight, mxfp8_linear
-from .weight import BlockwiseFp8Weight, BlockwiseMxfp8Weight, BlockwiseQuantWeight
+from .weight import BlockwiseFp8Weight, BlockwiseMxfp4Weight, BlockwiseMxfp8Weight, BlockwiseQuantWeight
 
 
 class PrequantizedLinearGemms(Protocol):
@@ -192,6 +193,28 @@ class FlexShardMxfp8BlockwiseLinear(FlexShardPrequantizedLinear):
         return mxfp8_linear(x, w, q, fwd, dgrad)
 
 
+class FlexShardMxfp4BlockwiseLinear(FlexShardPrequantizedLinear):
+    """Linear whose forward product runs on 4-bit operands (``kind::mxf4``): activations are quantised 1x32 on the fly, the
+    weight in 32x32 tiles. Gradients run on the 8-bit products, with the 4-bit weight's own values for the input's. The
+    master weight is quantised at every call; ``freeze_`` keeps the 4-bit payload in its place (scoring, a frozen teacher)."""
+
+    def payload(self, w):
+        if not isinstance(w, BlockwiseMxfp4Weight):
+            w = BlockwiseMxfp4Weight.from_float(w)
+        return w.qdata, w.scale, w.dgrad_scale
+
+    def freeze_(self) -> "FlexShardMxfp4BlockwiseLinear":
+        """Replaces the master weight by its 4-bit payload, which takes no gradient."""
+        if not isinstance(self.weight, BlockwiseMxfp4Weight):
+            self.weight = nn.Parameter(BlockwiseMxfp4Weight.from_float(self.weight), requires_grad=False)
+        return self
+
+    def forward(self, x):
+        w = self.weight
+        q, fwd, dgrad = self.payload(w)
+        return mxfp4_linear(x, None if isinstance(w, BlockwiseMxfp4Weight) else w, q, fwd, dgrad)
+
+
 def _eligible(child) -> bool:
     return (isinstance(child, nn.Linear) and child.bias is None and child.in_features % 128 == 0
             and child.out_features % 128 == 0)
@@ -202,10 +225,10 @@ def convert_to_flex_shard_prequantized_linear(module: nn.Module, linear_cls: typ
                                               **from_float_kwargs) -> nn.Module:
     """Replace the ``nn.Linear`` children that ``filter_fn(dotted name, linear)`` selects (default: all) by
     ``linear_cls.from_float(linear, **from_float_kwargs)``, keeping the weights.  ``linear_cls`` defaults to the FP8
-    blockwise layer; this library's two layers only take bias-free layers whose dims are multiples of 128 and skip
+    blockwise layer; this library's three layers only take bias-free layers whose dims are multiples of 128 and skip
     the others.  Parity: ``blockwise_quant/linear.py:158-184`` of the reference."""
     linear_cls = linear_cls or FlexShardFloat8BlockwiseLinear
-    own = linear_cls in (FlexShardFloat8BlockwiseLinear, FlexShardMxfp8BlockwiseLinear)
+    own = linear_cls in (FlexShardFloat8BlockwiseLinear, FlexShardMxfp8BlockwiseLinear, FlexShardMxfp4BlockwiseLinear)
 
     def walk(parent: nn.Module, prefix: str) -> None:
         for name, child in list(parent.named_children()):
@@ -225,6 +248,11 @@ def convert_to_flex_shard_prequantized_linear(module: nn.Module, linear_cls: typ
 def convert_to_flex_shard_mxfp8_blockwise_linear(module: nn.Module, filter_fn=None) -> nn.Module:
     """Replace bias-free ``nn.Linear`` layers whose dims are multiples of 128 by the MXFP8 linear."""
     return convert_to_flex_shard_prequantized_linear(module, FlexShardMxfp8BlockwiseLinear, filter_fn)
+
+
+def convert_to_flex_shard_mxfp4_blockwise_linear(module: nn.Module, filter_fn=None) -> nn.Module:
+    """Replace bias-free ``nn.Linear`` layers whose dims are multiples of 128 by the MXFP4 linear."""
+    return convert_to_flex_shard_prequantized_linear(module, FlexShardMxfp4BlockwiseLinear, filter_fn)
 
 
 def convert_to_flex_shard_float8_blockwise_linear(module: nn.Module, filter_fn=None) -> nn.Module:

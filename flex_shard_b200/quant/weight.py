@@ -123,6 +123,42 @@ class BlockwiseMxfp8Weight(BlockwiseQuantWeight):
                                                         te[flat * out // 32:(flat + 1) * out // 32], (out, cin), self.dtype)
 
 
+class BlockwiseMxfp4Weight(BlockwiseQuantWeight):
+    """MXFP4 weight: packed e2m1 codes ``[out, in / 2]`` with 32x32 tile scales, kept as the tile exponents plus the two
+    blocked scale tensors the tensor core reads (``scale``: groups along ``in`` for y = x W^T; ``dgrad_scale``: groups
+    along ``out`` for dx = dy W). Made from a high-precision matrix; ``linear`` and the prequantised layers consume it."""
+
+    inner_names = ("qdata", "scale", "dgrad_scale")
+
+    @staticmethod
+    def __new__(cls, qdata, scale, shape, dtype=torch.bfloat16, dgrad_scale=None, **extra):
+        r = BlockwiseQuantWeight.__new__(cls, qdata, scale, shape, dtype, **extra)
+        r.dgrad_scale = dgrad_scale
+        return r
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor) -> "BlockwiseMxfp4Weight":
+        from ..ops.mxfp4 import mx4_quantize_weight_operands
+
+        if isinstance(w, BlockwiseQuantWeight):
+            raise ValueError("the weight is quantised already")
+        q, e, fwd, dgrad = mx4_quantize_weight_operands(w.detach())
+        return cls(q, fwd, w.shape, w.dtype, dgrad_scale=dgrad, tile_exp=e)
+
+    @classmethod
+    def __tensor_unflatten__(cls, inner, meta, outer_size=None, outer_stride=None):
+        return cls(inner["qdata"], inner["scale"], meta["shape"], meta["dtype"], dgrad_scale=inner["dgrad_scale"],
+                   **meta.get("extra", {}))
+
+    def _rebuild(self):
+        return type(self)(self.qdata, self.scale, self.shape, self.dtype, dgrad_scale=self.dgrad_scale, **self.extra)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        from ..ops.mxfp4 import mx4_dequantize
+
+        return mx4_dequantize(self.qdata, self.scale, torch.float32).to(dtype)
+
+
 def blockwise_mxfp8_dequant_weight(fp8_data: torch.Tensor, fwd_scale: torch.Tensor) -> torch.Tensor:
     """Row-major e4m3 data with its forward-orientation blocked scales -> fp32."""
     from ..ops.mxfp8 import mx_dequantize
