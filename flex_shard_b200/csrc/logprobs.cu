@@ -38,7 +38,103 @@ __device__ __forceinline__ unsigned long long order_key(float v, int index) {
   return static_cast<unsigned long long>(value_key(v)) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
 }
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int MAX_CHUNKS = 8;       // chunk maxima a thread keeps
+constexpr int CAP = 1024;           // candidates a CTA keeps
+constexpr int MAX_PARTS = 8;        // CTAs of a row (a portable cluster)
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <typename T> struct Vec;     // 16 bytes: L elements
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int L = 8;
+  static constexpr uint32_t NEG_INF = 0xff80ff80u;
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[2 * j] = __uint_as_float(w[j] << 16);
+      f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+};
+template <> struct Vec<__half> {
+  static constexpr int L = 8;
+  static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = __half22float2(h[j]);
+      f[2 * j] = a.x;
+      f[2 * j + 1] = a.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    uint4 v;
+    __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+    return v;
+  }
+};
+template <> struct Vec<float> {
+  static constexpr int L = 4;
+  static constexpr uint32_t NEG_INF = 0xff800000u;
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+
+// A row as whole 16-byte vectors between a head and a tail of single elements.
+struct RowSpan {
+  int head, nvec, tail;
+};
+template <typename T>
+__device__ __forceinline__ RowSpan row_span(const T* r, int V) {
+  RowSpan s;
+  s.head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / static_cast<int>(sizeof(T)), V);
+  s.nvec = (V - s.head) / Vec<T>::L;
+  s.tail = V - s.head - s.nvec * Vec<T>::L;
+  return s;
+}
+
+// ------------------------------------------------------------------ sorted lists of a warp, largest first
+template <typename K>
+__device__ __forceinline__ K exchange(K v, int stride, bool keep_max) {
+  const K o = __shfl_xor_sync(0xffffffffu, v, stride);
+  return keep_max ? (o > v ? o : v) : (o < v ? o : v);
+}
+template <typename K>
+__device__ __forceinline__ K warp_sort(K v, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int stride = size >> 1; stride > 0; stride >>= 1) v = exchange(v, stride, ((lane & stride) == 0) == ((lane & size) == 0));
+  return v;
+}
+// The 32 largest of two sorted lists; `b` is handed in reversed.
+template <typename K>
+__device__ __forceinline__ K warp_merge(K a, K b_reversed, int lane) {
+  K v = a > b_reversed ? a : b_reversed;
+#pragma unroll
+  for (int stride = 16; stride > 0; stride >>= 1) v = exchange(v, stride, (lane & stride) == 0);
+  return v;
+}
 
 // Sum / maximum over the block, in every thread; the order of the additions is fixed.
 template <typename F>
@@ -48,60 +144,129 @@ __device__ __forceinline__ float block_reduce(float v, float* red, F op) {
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = red[threadIdx.x & (THREADS / 32 - 1)];
+  v = red[threadIdx.x & (WARPS - 1)];
 #pragma unroll
-  for (int o = THREADS / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = WARPS / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
-// One CTA per row: maximum, sums, then the alternatives one after the other.
+// Running sums relative to a maximum m, in base 2: s = sum 2^((x - m) c), u = sum (x - m) c 2^((x - m) c), c = log2(e) / temperature.
+struct Sums {
+  float m, s, u;
+  __device__ __forceinline__ void raise(float to, float c) {
+    const float d = (m - to) * c, f = ex2(d);
+    u = (u + s * d) * f;
+    s *= f;
+    m = to;
+  }
+};
+
+struct Smem {
+  float red[WARPS];
+  float part[MAX_PARTS][4];                       // m, s, u of the row's parts (in the first CTA)
+  unsigned long long lists[MAX_PARTS][32];        // their alternatives
+  unsigned long long cand[CAP];
+  uint32_t keys[WARPS][32];
+  float cmax[MAX_CHUNKS][THREADS];
+  uint32_t bound;
+  int count;
+};
+
+// The alternatives of this CTA's part [lo, hi), in warp 0's registers: lane i has the i-th largest key (0: none). Elements that
+// can be among the k largest are at least as large as the k-th largest of the threads' maxima; they are collected from the
+// chunks whose maximum says that they have some, and sorted. Random logits leave little more than k of them. Where there are
+// more than fit (masked or equal logits), those above the bound are collected and those equal to it counted off from the
+// lowest index; where even the former do not fit, k maxima are taken one after the other.
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
-                long long ignore_index, float* __restrict__ logprob, float* __restrict__ entropy, float2* __restrict__ stats,
-                float* __restrict__ top_lp, long long* __restrict__ top) {
-  __shared__ float red[THREADS / 32];
-  __shared__ unsigned long long best[THREADS / 32];
-  const long long row = blockIdx.x;
-  const T* r = x + row * ld;
-  const long long tgt = target[row];
-  const int tid = threadIdx.x;
-  if (tgt == ignore_index) {
-    if (tid == 0) {
-      logprob[row] = entropy[row] = 0.f;
-      stats[row] = make_float2(0.f, 0.f);
-    }
-    if (tid < k) {
-      top_lp[row * k + tid] = 0.f;
-      top[row * k + tid] = -1;
-    }
-    return;
-  }
-  float m = -INFINITY;
-  for (int i = tid; i < V; i += THREADS) m = max_nan(m, to_f(r[i]));
-  m = block_reduce(m, red, [](float a, float b) { return max_nan(a, b); });
-  float s = 0.f, u = 0.f;
-  for (int i = tid; i < V; i += THREADS) {
-    const float d = (to_f(r[i]) - m) * inv_t;
-    if (d != -INFINITY) {
-      const float e = __expf(d);
-      s += e;
-      u += d * e;
+__device__ __noinline__ unsigned long long part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at,
+                                                    float tmax, int cl, int k, int lo, int hi, Smem& sm) {
+  constexpr int L = Vec<T>::L;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t v = warp_sort(value_key(tmax), lane);
+  sm.keys[warp][lane] = v;
+  if (tid == 0) sm.count = 0;
+#pragma unroll
+  for (int w = WARPS / 2; w > 0; w >>= 1) {
+    __syncthreads();
+    if (warp < w) {
+      v = warp_merge(v, sm.keys[warp + w][31 - lane], lane);
+      sm.keys[warp][lane] = v;
     }
   }
-  auto add = [](float a, float b) { return a + b; };
-  s = block_reduce(s, red, add);
-  u = block_reduce(u, red, add);
-  const float log_s = logf(s);
-  if (tid == 0) {
-    logprob[row] = tgt >= 0 && tgt < V ? (to_f(r[tgt]) - m) * inv_t - log_s : __uint_as_float(0x7fc00000u);
-    entropy[row] = log_s - u / s;
-    stats[row] = make_float2(m, log_s);
+  if (tid == k - 1) sm.bound = v;
+  __syncthreads();
+  const uint32_t bound = sm.bound;
+  auto collect = [&](uint32_t least) {
+    if (value_key(tmax) >= least) {
+      if (edge_at >= 0 && value_key(edge) >= least) {
+        const int slot = atomicAdd(&sm.count, 1);
+        if (slot < CAP) sm.cand[slot] = order_key(edge, edge_at);
+      }
+      const int n = first_vec + tid < end_vec ? (end_vec - first_vec - tid + THREADS - 1) / THREADS : 0;
+      for (int ch = 0; ch * cl < n; ++ch) {
+        if (value_key(sm.cmax[ch][tid]) < least) continue;
+        const int stop = min(n, (ch + 1) * cl);
+        for (int j = ch * cl; j < stop; ++j) {
+          const int vec = first_vec + tid + j * THREADS;
+          float f[L];
+          Vec<T>::unpack(*reinterpret_cast<const uint4*>(r + head + static_cast<long long>(vec) * L), f);
+#pragma unroll
+          for (int q = 0; q < L; ++q)
+            if (value_key(f[q]) >= least) {
+              const int slot = atomicAdd(&sm.count, 1);
+              if (slot < CAP) sm.cand[slot] = order_key(f[q], head + vec * L + q);
+            }
+        }
+      }
+    }
+    __syncthreads();
+  };
+  auto sorted = [&](int n) {      // warp 0: the 32 largest of the candidates
+    unsigned long long best = 0;
+    for (int at = 0; at < n; at += 32) {
+      const unsigned long long b = warp_sort(at + lane < n ? sm.cand[at + lane] : 0ull, lane);
+      best = at == 0 ? b : warp_merge(best, __shfl_xor_sync(0xffffffffu, b, 31), lane);
+    }
+    return best;
+  };
+  collect(bound);
+  const int n = sm.count;
+  if (n <= CAP) return warp == 0 ? sorted(n) : 0ull;
+  __syncthreads();
+  if (tid == 0) sm.count = 0;
+  __syncthreads();
+  if (bound != 0xffffffffu) collect(bound + 1);
+  const int above = sm.count;
+  if (above <= CAP) {
+    const unsigned long long best = warp == 0 ? sorted(above) : 0ull;
+    __syncthreads();
+    int have = above;                                 // candidates so far; those equal to the bound follow in index order
+    if (warp == 0 && lane < min(above, 32)) sm.cand[lane] = best;
+    if (have < k) {
+      for (int base = lo; base < hi && have < k; base += THREADS) {
+        const int i = base + tid;
+        const bool eq = i < hi && value_key(to_f(r[i])) == bound;
+        const uint32_t votes = __ballot_sync(0xffffffffu, eq);
+        __syncthreads();
+        if (lane == 0) sm.keys[0][warp] = __popc(votes);
+        __syncthreads();
+        int before = have, all = have;
+        for (int w = 0; w < WARPS; ++w) {
+          if (w < warp) before += sm.keys[0][w];
+          all += sm.keys[0][w];
+        }
+        const int at = before + __popc(votes & ((1u << lane) - 1));
+        if (eq && at < 32) sm.cand[at] = order_key(to_f(r[i]), i);
+        have = all;
+      }
+    }
+    __syncthreads();
+    return warp == 0 && lane < have ? sm.cand[lane] : 0ull;
   }
-  unsigned long long last = ~0ull;
+  unsigned long long last = ~0ull, mine = 0;
   for (int c = 0; c < k; ++c) {
     unsigned long long b = 0;
-    for (int i = tid; i < V; i += THREADS) {
+    for (int i = lo + tid; i < hi; i += THREADS) {
       const unsigned long long key = order_key(to_f(r[i]), i);
       if (key < last && key > b) b = key;
     }
@@ -111,25 +276,187 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
       b = other > b ? other : b;
     }
     __syncthreads();
-    if ((tid & 31) == 0) best[tid >> 5] = b;
+    if (lane == 0) sm.cand[warp] = b;
     __syncthreads();
-    for (int w = 0; w < THREADS / 32; ++w) b = best[w] > b ? best[w] : b;
+    for (int w = 0; w < WARPS; ++w) b = sm.cand[w] > b ? sm.cand[w] : b;
     last = b;
-    if (tid == 0) {
-      const int at = static_cast<int>(0xffffffffu - static_cast<uint32_t>(b));
-      top[row * k + c] = at;
-      top_lp[row * k + c] = (to_f(r[at]) - m) * inv_t - log_s;
+    if (lane == c) mine = b;
+  }
+  return mine;
+}
+
+// One read of the logits: a row, or a part of it where there are few rows (the CTAs of a cluster then leave their sums and
+// alternatives with the first one). Every thread keeps a running maximum and sums relative to it, and the maxima of its chunks
+// for the alternatives.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS)
+logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
+                long long ignore_index, int parts, float* __restrict__ logprob, float* __restrict__ entropy,
+                float2* __restrict__ stats, float* __restrict__ top_lp, long long* __restrict__ top) {
+  constexpr int L = Vec<T>::L;
+  __shared__ Smem sm;
+  const long long row = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x % parts);
+  const T* r = x + row * ld;
+  const long long tgt = target[row];
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tgt == ignore_index) {                         // the same for every CTA of the row: none of them meets a barrier
+    if (part == 0) {
+      if (tid == 0) {
+        logprob[row] = entropy[row] = 0.f;
+        stats[row] = make_float2(0.f, 0.f);
+      }
+      if (tid < k) {
+        top_lp[row * k + tid] = 0.f;
+        top[row * k + tid] = -1;
+      }
     }
+    return;
+  }
+  if (parts > 1) cluster_arrive();                   // waited for before the exchange
+  const bool inside = tgt >= 0 && tgt < V;
+  const float xt = part == 0 && tid == 0 && inside ? to_f(r[tgt]) : 0.f;
+  const float c = inv_t * L2E;
+  // Sums start at a finite maximum: a row whose maximum is not above it, or overflows when scaled, or whose sum is not a
+  // finite number, is done again at the end, with differences taken before they are scaled.
+  const float floor_ = fmaxf(-1e38f / c, -3e38f);
+  const RowSpan span = row_span(r, V);
+  const int per = (span.nvec + parts - 1) / parts;
+  const int first_vec = min(part * per, span.nvec), end_vec = min(first_vec + per, span.nvec);
+  const int n = (end_vec - first_vec + THREADS - 1) / THREADS;      // vectors of a thread
+  const int cl = max(4, ((n + MAX_CHUNKS - 1) / MAX_CHUNKS + 3) / 4 * 4);
+  Sums a{floor_, 0.f, 0.f};
+  float tmax = -INFINITY, cmax = -INFINITY;
+  auto take = [&](const uint4& v) {
+    float f[L];
+    Vec<T>::unpack(v, f);
+    float vm = f[0];
+#pragma unroll
+    for (int j = 1; j < L; ++j) vm = max_nan(vm, f[j]);
+    cmax = max_nan(cmax, vm);
+    if (vm > a.m) a.raise(vm, c);
+    const float mo = -a.m * c;
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const float d = max_nan(fmaf(f[j], c, mo), -256.f), e = ex2(d);   // 2^-256 is 0: nothing from masked tokens
+      a.s += e;
+      a.u = fmaf(d, e, a.u);
+    }
+  };
+  const uint4* g = reinterpret_cast<const uint4*>(r + span.head);
+  const uint4 none = make_uint4(Vec<T>::NEG_INF, Vec<T>::NEG_INF, Vec<T>::NEG_INF, Vec<T>::NEG_INF);
+  int chunk = 0, in_chunk = 0;
+  for (int i = first_vec + tid; i < end_vec; i += 4 * THREADS) {
+    uint4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = i + q * THREADS < end_vec ? load_stream(g + i + q * THREADS) : none;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) take(v[q]);
+    if (TOP) {
+      in_chunk += 4;
+      if (in_chunk == cl) {
+        sm.cmax[chunk++][tid] = cmax;
+        tmax = max_nan(tmax, cmax);
+        cmax = -INFINITY;
+        in_chunk = 0;
+      }
+    }
+  }
+  if (TOP) {
+    if (in_chunk) sm.cmax[chunk][tid] = cmax;
+    tmax = max_nan(tmax, cmax);
+  }
+  // the elements before and after the vectors, one a thread
+  const int edges = (part == 0 ? span.head : 0) + (part == parts - 1 ? span.tail : 0);
+  float edge = -INFINITY;
+  int edge_at = -1;
+  if (tid < edges) {
+    edge_at = part == 0 && tid < span.head ? tid : V - edges + tid;
+    edge = to_f(r[edge_at]);
+    tmax = max_nan(tmax, edge);
+    if (edge > a.m) a.raise(edge, c);
+    const float d = max_nan(fmaf(edge, c, -a.m * c), -256.f), e = ex2(d);
+    a.s += e;
+    a.u = fmaf(d, e, a.u);
+  }
+  const float m = block_reduce(a.m, sm.red, [](float p, float q) { return fmaxf(p, q); });
+  a.raise(m, c);
+  auto add = [](float p, float q) { return p + q; };
+  Sums all{m, block_reduce(a.s, sm.red, add), block_reduce(a.u, sm.red, add)};
+  unsigned long long best = 0;
+  if constexpr (TOP) {
+    const int lo = part == 0 ? 0 : span.head + first_vec * L, hi = part == parts - 1 ? V : span.head + end_vec * L;
+    best = part_top(r, first_vec, end_vec, span.head, edge, edge_at, tmax, cl, k, lo, hi, sm);
+  }
+  if (parts > 1) {
+    cluster_wait();                                  // every CTA of the cluster has started: the first one's memory is there
+    if (tid < 32) {
+      const uint32_t dst = map_to_cta(smem_u32(&sm.part[part][0]), 0);
+      if (lane == 0) {
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(all.m) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(all.s) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(all.u) : "memory");
+      }
+      if (TOP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_cta(smem_u32(&sm.lists[part][lane]), 0)), "l"(best) : "memory");
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (part != 0) return;
+    float top_m = sm.part[0][0];
+    for (int p = 1; p < parts; ++p) top_m = fmaxf(top_m, sm.part[p][0]);
+    all = Sums{top_m, 0.f, 0.f};
+    for (int p = 0; p < parts; ++p) {
+      Sums o{sm.part[p][0], sm.part[p][1], sm.part[p][2]};
+      o.raise(top_m, c);
+      all.s += o.s;
+      all.u += o.u;
+    }
+    if (TOP && tid < 32)
+      for (int p = 1; p < parts; ++p) best = warp_merge(best, sm.lists[p][31 - lane], lane);
+  }
+  float log_s = logf(all.s), H = log_s - all.u * LN2 / all.s;
+  if (!(all.m > floor_ && fabsf(all.m * c) < 1e38f && fabsf(all.s) < INFINITY)) {      // the same in all threads
+    float mx = -INFINITY;
+    for (int i = tid; i < V; i += THREADS) mx = max_nan(mx, to_f(r[i]));
+    mx = block_reduce(mx, sm.red, [](float p, float q) { return max_nan(p, q); });
+    float s = 0.f, u = 0.f;
+    for (int i = tid; i < V; i += THREADS) {
+      const float d = (to_f(r[i]) - mx) * inv_t;
+      if (d != -INFINITY) {
+        const float e = __expf(d);
+        s += e;
+        u += e == 0.f ? 0.f : d * e;
+      }
+    }
+    s = block_reduce(s, sm.red, add);
+    u = block_reduce(u, sm.red, add);
+    all.m = mx;
+    log_s = logf(s);
+    H = log_s - u / s;
+  }
+  if (tid == 0) {
+    logprob[row] = inside ? (xt - all.m) * inv_t - log_s : __uint_as_float(0x7fc00000u);
+    entropy[row] = H;
+    stats[row] = make_float2(all.m, log_s);
+  }
+  if (TOP && tid < k) {
+    const int at = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+    const uint32_t key = static_cast<uint32_t>(best >> 32);
+    const float v = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    top[row * k + tid] = at;
+    top_lp[row * k + tid] = (v - all.m) * inv_t - log_s;
   }
 }
 
 // dx_j = [ -p_j (G + gH (log p_j + H)) + g [j = target] + sum_i g_i [j = top_i] ] / temperature, G = g + sum_i g_i.
+// Row blockIdx.x, part blockIdx.y. With l = log2 p_j the first term is p_j (l A + B); the chosen positions are written again.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
                     long long ignore_index, const long long* __restrict__ top, const float2* __restrict__ stats,
                     const float* __restrict__ entropy, const float* __restrict__ glp, const float* __restrict__ gh,
                     const float* __restrict__ gtop, T* __restrict__ dx, long long ldd) {
+  constexpr int L = Vec<T>::L;
   const long long row = blockIdx.x;
   const T* r = x + row * ld;
   T* d = dx + row * ldd;
@@ -140,31 +467,83 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ targe
   float G = g;
   bool any = g != 0.f || h != 0.f;
   if (gtop && !ignored)
-    for (int c = 0; c < k; ++c) {
-      G += gtop[row * k + c];
-      any |= gtop[row * k + c] != 0.f;
+    for (int i = 0; i < k; ++i) {
+      G += gtop[row * k + i];
+      any |= gtop[row * k + i] != 0.f;
     }
-  if (!any) {
-    for (int i = tid; i < V; i += THREADS) d[i] = from_f<T>(0.f);
-    return;
-  }
   if (tgt < 0 || tgt >= V) G += g * __uint_as_float(0x7fc00000u);      // a target outside the vocabulary: NaN
-  const float m = stats[row].x, log_s = stats[row].y, H = entropy[row];
+  const float2 st = stats[row];
+  const float m = st.x, log_s = st.y, H = entropy[row], c = inv_t * L2E;
+  const float A = -h * LN2 * inv_t, B = -(G + h * H) * inv_t;
+  // scaled maxima that overflow: differences first, as in the forward pass
+  const bool wide = !(fabsf(m * c) < 1e38f);
+  const float mo = -m * c - log_s * L2E;
   auto smooth = [&](float v) {
-    const float lp = (v - m) * inv_t - log_s, p = __expf(lp);
-    return p == 0.f ? 0.f * G : -p * (G + h * (lp + H));
+    const float l = max_nan(wide ? (v - m) * c - log_s * L2E : fmaf(v, c, mo), -256.f);
+    return ex2(l) * fmaf(l, A, B);
   };
-  for (int i = tid; i < V; i += THREADS) d[i] = from_f<T>(smooth(to_f(r[i])) * inv_t);
+  const RowSpan span = row_span(r, V);
+  const bool vec = ((reinterpret_cast<uintptr_t>(r) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  const int parts = gridDim.y, part = blockIdx.y;
+  int lo, hi;                                         // elements of this CTA
+  if (vec) {
+    const int per = (span.nvec + parts - 1) / parts;
+    const int first = min(part * per, span.nvec), end = min(first + per, span.nvec);
+    lo = part == 0 ? 0 : span.head + first * L;
+    hi = part == parts - 1 ? V : span.head + end * L;
+    const uint4* src = reinterpret_cast<const uint4*>(r + span.head);
+    uint4* dst = reinterpret_cast<uint4*>(d + span.head);
+    if (!any) {
+      for (int i = first + tid; i < end; i += THREADS) dst[i] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int i = first + tid; i < end; i += 4 * THREADS) {
+        uint4 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i + q * THREADS < end) v[q] = load_stream(src + i + q * THREADS);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (i + q * THREADS >= end) continue;
+          float f[L];
+          Vec<T>::unpack(v[q], f);
+#pragma unroll
+          for (int j = 0; j < L; ++j) f[j] = smooth(f[j]);
+          dst[i + q * THREADS] = Vec<T>::pack(f);
+        }
+      }
+    }
+    const int edges = (part == 0 ? span.head : 0) + (part == parts - 1 ? span.tail : 0);
+    if (tid < edges) {
+      const int at = part == 0 && tid < span.head ? tid : V - edges + tid;
+      d[at] = from_f<T>(any ? smooth(to_f(r[at])) : 0.f);
+    }
+  } else {
+    const int per = (V + parts - 1) / parts;
+    lo = min(part * per, V);
+    hi = min(lo + per, V);
+    for (int i = lo + tid; i < hi; i += THREADS) d[i] = from_f<T>(any ? smooth(to_f(r[i])) : 0.f);
+  }
+  if (!any) return;
   __syncthreads();
   // the chosen positions again, with what they get besides: alternatives differ from one another, the target may be one
-  bool taken = false;
-  if (gtop)
-    for (int c = 0; c < k; ++c) taken |= top[row * k + c] == tgt;
-  if (tid < k && gtop) {
+  if (gtop && tid < k) {
     const long long at = top[row * k + tid];
-    d[at] = from_f<T>((smooth(to_f(r[at])) + gtop[row * k + tid] + (at == tgt ? g : 0.f)) * inv_t);
+    if (at >= lo && at < hi)
+      d[at] = from_f<T>(smooth(to_f(r[at])) + (gtop[row * k + tid] + (at == tgt ? g : 0.f)) * inv_t);
   }
-  if (tid == MAX_TOP && !taken && tgt >= 0 && tgt < V) d[tgt] = from_f<T>((smooth(to_f(r[tgt])) + g) * inv_t);
+  if (tid == MAX_TOP && tgt >= lo && tgt < hi) {
+    bool taken = false;
+    if (gtop)
+      for (int i = 0; i < k; ++i) taken |= top[row * k + i] == tgt;
+    if (!taken) d[tgt] = from_f<T>(smooth(to_f(r[tgt])) + g * inv_t);
+  }
+}
+
+// CTAs of a row: enough to fill the SMs twice, but at least 4096 elements each.
+int row_parts(long long T, int V) {
+  int parts = 1;
+  while (parts < MAX_PARTS && T * parts * 2 <= 296 && V / (parts * 2) >= 4096) parts *= 2;
+  return parts;
 }
 
 inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH; }
@@ -178,10 +557,26 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
   if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2) return FSB_ERR_BAD_ARG;
   if (T > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   if (T == 0) return FSB_OK;
+  const int parts = row_parts(T, V);
+  if (T * parts > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(T * parts), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = parts;
+  at.val.clusterDim.y = 1;
+  at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   auto run = [&](auto* p) {
-    logprobs_kernel<<<static_cast<unsigned>(T), THREADS, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, logprob, entropy,
-                                                                      static_cast<float2*>(stats), top_lp, top);
-    return ok();
+    using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    auto kernel = k > 0 ? logprobs_kernel<E, true> : logprobs_kernel<E, false>;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p, target, V, ld, inv_t, k, ignore_index, parts, logprob, entropy,
+                                               static_cast<float2*>(stats), top_lp, top);
+    const int rc = ok();   // also clears the error of a launch that failed
+    return err == cudaSuccess ? rc : static_cast<int>(FSB_ERR_LAUNCH);
   };
   if (kind == 0) return run(static_cast<const __nv_bfloat16*>(x));
   if (kind == 1) return run(static_cast<const __half*>(x));
@@ -198,7 +593,8 @@ FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* tar
   if (T == 0) return FSB_OK;
   auto run = [&](auto* p) {
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    logprobs_bwd_kernel<<<static_cast<unsigned>(T), THREADS, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
+    const dim3 grid(static_cast<unsigned>(T), row_parts(T, V));
+    logprobs_bwd_kernel<<<grid, THREADS, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
                                                                           static_cast<const float2*>(stats), entropy, glp, gh, gtop, static_cast<E*>(dx), ldd);
     return ok();
   };

@@ -35,7 +35,10 @@ def check(x, t, temperature=1.0, k=0, grads=True, seed=1):
     want, size = gradient(before, t, temperature, k, gl, gh, gt)
     assert dx.shape == x.shape and dx.dtype == x.dtype
     off = (dx.double() - want).abs()
-    bound = want.abs() * HALF_STEP[x.dtype] + size * 8 * tol * (1 + math.log(V)) + SMALLEST[x.dtype]
+    # A probability below 2^-126 (log probability below -87.4) counts as 0: p (G + h (log p + H)), which falls with p there, is
+    # then missing, at most 2^-126 (|G| + |h| (88 + ln V)).
+    lost = 2.0 ** -126 * (gl.abs() + gt.abs().sum(1) + gh.abs() * (88 + math.log(V)))[:, None] / temperature
+    bound = want.abs() * HALF_STEP[x.dtype] + size * 8 * tol * (1 + math.log(V)) + SMALLEST[x.dtype] + lost
     good = want.isfinite().all(1)
     assert (off <= bound)[good].all(), float((off - bound)[good].max())
     assert dx[~good].isnan().all()
