@@ -34,13 +34,14 @@ __device__ __forceinline__ uint32_t value_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ unsigned long long order_key(float v, int index) {
   return static_cast<unsigned long long>(value_key(v)) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
 }
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_CHUNKS = 8;       // chunk maxima a thread keeps
-constexpr int CAP = 1024;           // candidates a CTA keeps
+constexpr int GROUPS = 64;          // groups of threads whose maxima bound the alternatives
+constexpr int CAP = 512;            // candidates a CTA keeps
 constexpr int MAX_PARTS = 8;        // CTAs of a row (a portable cluster)
 
 __device__ __forceinline__ float ex2(float v) {
@@ -57,6 +58,11 @@ template <typename T> struct Vec;     // 16 bytes: L elements
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int L = 8;
   static constexpr uint32_t NEG_INF = 0xff80ff80u;
+  static __device__ __forceinline__ float largest(const uint4& v) {   // a NaN if there is one
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const float2 m = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(m.x, m.y);
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -72,6 +78,11 @@ template <> struct Vec<__nv_bfloat16> {
 template <> struct Vec<__half> {
   static constexpr int L = 8;
   static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const float2 m = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(m.x, m.y);
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
@@ -92,6 +103,9 @@ template <> struct Vec<__half> {
 template <> struct Vec<float> {
   static constexpr int L = 4;
   static constexpr uint32_t NEG_INF = 0xff800000u;
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
   }
@@ -113,32 +127,10 @@ __device__ __forceinline__ RowSpan row_span(const T* r, int V) {
   return s;
 }
 
-// ------------------------------------------------------------------ sorted lists of a warp, largest first
-template <typename K>
-__device__ __forceinline__ K exchange(K v, int stride, bool keep_max) {
-  const K o = __shfl_xor_sync(0xffffffffu, v, stride);
-  return keep_max ? (o > v ? o : v) : (o < v ? o : v);
-}
-template <typename K>
-__device__ __forceinline__ K warp_sort(K v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int stride = size >> 1; stride > 0; stride >>= 1) v = exchange(v, stride, ((lane & stride) == 0) == ((lane & size) == 0));
-  return v;
-}
-// The 32 largest of two sorted lists; `b` is handed in reversed.
-template <typename K>
-__device__ __forceinline__ K warp_merge(K a, K b_reversed, int lane) {
-  K v = a > b_reversed ? a : b_reversed;
-#pragma unroll
-  for (int stride = 16; stride > 0; stride >>= 1) v = exchange(v, stride, (lane & stride) == 0);
-  return v;
-}
-
 // Sum / maximum over the block, in every thread; the order of the additions is fixed.
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ float block_reduce(float v, float* red, F op) {
+  constexpr int WARPS = THREADS / 32;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   __syncthreads();
@@ -161,109 +153,128 @@ struct Sums {
   }
 };
 
-struct Smem {
-  float red[WARPS];
-  float part[MAX_PARTS][4];                       // m, s, u of the row's parts (in the first CTA)
-  unsigned long long lists[MAX_PARTS][32];        // their alternatives
+template <int THREADS>
+struct SumsSmem {
+  float red[32];
+  float warp[THREADS / 32][3];                    // m, s, u of the warps
+  float part[MAX_PARTS][3];                       // ... and of the row's parts (in the first CTA)
+};
+template <int THREADS>
+struct TopSmem {
+  unsigned long long lists[MAX_PARTS * 32];       // sorted alternatives of the row's parts (in the first CTA; 0: none)
+  unsigned long long best[32];                    // ... of this part, then of the row
   unsigned long long cand[CAP];
-  uint32_t keys[WARPS][32];
+  uint32_t groups[GROUPS];
   float cmax[MAX_CHUNKS][THREADS];
+  uint16_t work[MAX_CHUNKS * THREADS];
   uint32_t bound;
-  int count;
+  int count[4];
 };
 
-// The alternatives of this CTA's part [lo, hi), in warp 0's registers: lane i has the i-th largest key (0: none). Elements that
-// can be among the k largest are at least as large as the k-th largest of the threads' maxima; they are collected from the
-// chunks whose maximum says that they have some, and sorted. Random logits leave little more than k of them. Where there are
-// more than fit (masked or equal logits), those above the bound are collected and those equal to it counted off from the
-// lowest index; where even the former do not fit, k maxima are taken one after the other.
-template <typename T>
-__device__ __noinline__ unsigned long long part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at,
-                                                    float tmax, int cl, int k, int lo, int hi, Smem& sm) {
-  constexpr int L = Vec<T>::L;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint32_t v = warp_sort(value_key(tmax), lane);
-  sm.keys[warp][lane] = v;
-  if (tid == 0) sm.count = 0;
-#pragma unroll
-  for (int w = WARPS / 2; w > 0; w >>= 1) {
-    __syncthreads();
-    if (warp < w) {
-      v = warp_merge(v, sm.keys[warp + w][31 - lane], lane);
-      sm.keys[warp][lane] = v;
-    }
+// Keys of `from`[0, n), all different but for zeros (none), put in order, largest first: rank by counting, the n keys read as
+// broadcasts. `to` has 32 places, zeroed before.
+template <int THREADS>
+__device__ __forceinline__ void rank_keys(const unsigned long long* from, int n, unsigned long long* to) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const unsigned long long mine = from[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += from[j] > mine ? 1 : 0;
+    if (rank < 32 && mine != 0) to[rank] = mine;
   }
-  if (tid == k - 1) sm.bound = v;
+}
+
+// The alternatives of this CTA's part [lo, hi) in sm.best (largest first, 0: none). Elements that can be among the k largest are
+// at least as large as the k-th largest of the maxima of 64 groups of threads; they are collected from the chunks whose maximum
+// says that they have some, and ranked. Random logits leave k to 1.5 k of them. Where there are more than fit (masked or equal
+// logits), those above the bound are collected and those equal to it counted off from the lowest index; where even the former
+// do not fit, k maxima are taken one after the other.
+template <typename T, int THREADS>
+__device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at, float tmax, int cl,
+                                      int k, int lo, int hi, TopSmem<THREADS>& sm) {
+  constexpr int L = Vec<T>::L, WARPS = THREADS / 32, PER = THREADS / GROUPS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t own = value_key(tmax);
+  uint32_t v = own;
+#pragma unroll
+  for (int o = PER / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (tid % PER == 0) sm.groups[tid / PER] = v;
+  if (tid < 32) sm.best[tid] = 0;
+  if (tid < 4) sm.count[tid] = 0;
+  __syncthreads();
+  if (tid < GROUPS) {
+    const uint32_t mine = sm.groups[tid];
+    int rank = 0;
+#pragma unroll 16
+    for (int j = 0; j < GROUPS; ++j) {
+      const uint32_t o = sm.groups[j];
+      rank += o > mine || (o == mine && j < tid) ? 1 : 0;
+    }
+    if (rank == k - 1) sm.bound = mine;
+  }
   __syncthreads();
   const uint32_t bound = sm.bound;
-  auto collect = [&](uint32_t least) {
-    if (value_key(tmax) >= least) {
-      if (edge_at >= 0 && value_key(edge) >= least) {
-        const int slot = atomicAdd(&sm.count, 1);
-        if (slot < CAP) sm.cand[slot] = order_key(edge, edge_at);
+  // Two steps, so that a warp does not walk the chunks of its lanes one after the other: the chunks that hold something go on a
+  // list, then every thread takes vectors of listed chunks.
+  auto collect = [&](uint32_t least, int& chunks, int& count) {
+    const float lf = key_value(least);
+    auto offer = [&](float f, int at) {
+      if (!(f < lf) && value_key(f) >= least) {
+        const int slot = atomicAdd(&count, 1);
+        if (slot < CAP) sm.cand[slot] = order_key(f, at);
       }
+    };
+    if (own >= least) {
+      if (edge_at >= 0) offer(edge, edge_at);
       const int n = first_vec + tid < end_vec ? (end_vec - first_vec - tid + THREADS - 1) / THREADS : 0;
-      for (int ch = 0; ch * cl < n; ++ch) {
-        if (value_key(sm.cmax[ch][tid]) < least) continue;
-        const int stop = min(n, (ch + 1) * cl);
-        for (int j = ch * cl; j < stop; ++j) {
-          const int vec = first_vec + tid + j * THREADS;
-          float f[L];
-          Vec<T>::unpack(*reinterpret_cast<const uint4*>(r + head + static_cast<long long>(vec) * L), f);
+      for (int ch = 0; ch * cl < n; ++ch)
+        if (value_key(sm.cmax[ch][tid]) >= least) sm.work[atomicAdd(&chunks, 1)] = static_cast<uint16_t>(ch * THREADS + tid);
+    }
+    __syncthreads();
+    const int units = chunks * cl;
+    for (int i = tid; i < units; i += THREADS) {
+      const int item = i / cl, w = sm.work[item];
+      const int vec = first_vec + w % THREADS + (w / THREADS * cl + i - item * cl) * THREADS;
+      if (vec >= end_vec) continue;
+      float f[L];
+      Vec<T>::unpack(*reinterpret_cast<const uint4*>(r + head + static_cast<long long>(vec) * L), f);
 #pragma unroll
-          for (int q = 0; q < L; ++q)
-            if (value_key(f[q]) >= least) {
-              const int slot = atomicAdd(&sm.count, 1);
-              if (slot < CAP) sm.cand[slot] = order_key(f[q], head + vec * L + q);
-            }
-        }
-      }
+      for (int e = 0; e < L; ++e) offer(f[e], head + vec * L + e);
     }
     __syncthreads();
   };
-  auto sorted = [&](int n) {      // warp 0: the 32 largest of the candidates
-    unsigned long long best = 0;
-    for (int at = 0; at < n; at += 32) {
-      const unsigned long long b = warp_sort(at + lane < n ? sm.cand[at + lane] : 0ull, lane);
-      best = at == 0 ? b : warp_merge(best, __shfl_xor_sync(0xffffffffu, b, 31), lane);
-    }
-    return best;
-  };
-  collect(bound);
-  const int n = sm.count;
-  if (n <= CAP) return warp == 0 ? sorted(n) : 0ull;
-  __syncthreads();
-  if (tid == 0) sm.count = 0;
-  __syncthreads();
-  if (bound != 0xffffffffu) collect(bound + 1);
-  const int above = sm.count;
-  if (above <= CAP) {
-    const unsigned long long best = warp == 0 ? sorted(above) : 0ull;
+  collect(bound, sm.count[0], sm.count[1]);
+  const int n = sm.count[1];
+  if (n <= CAP) {
+    rank_keys<THREADS>(sm.cand, n, sm.best);
     __syncthreads();
-    int have = above;                                 // candidates so far; those equal to the bound follow in index order
-    if (warp == 0 && lane < min(above, 32)) sm.cand[lane] = best;
-    if (have < k) {
-      for (int base = lo; base < hi && have < k; base += THREADS) {
-        const int i = base + tid;
-        const bool eq = i < hi && value_key(to_f(r[i])) == bound;
-        const uint32_t votes = __ballot_sync(0xffffffffu, eq);
-        __syncthreads();
-        if (lane == 0) sm.keys[0][warp] = __popc(votes);
-        __syncthreads();
-        int before = have, all = have;
-        for (int w = 0; w < WARPS; ++w) {
-          if (w < warp) before += sm.keys[0][w];
-          all += sm.keys[0][w];
-        }
-        const int at = before + __popc(votes & ((1u << lane) - 1));
-        if (eq && at < 32) sm.cand[at] = order_key(to_f(r[i]), i);
-        have = all;
-      }
-    }
-    __syncthreads();
-    return warp == 0 && lane < have ? sm.cand[lane] : 0ull;
+    return;
   }
-  unsigned long long last = ~0ull, mine = 0;
+  if (bound != 0xffffffffu) collect(bound + 1, sm.count[2], sm.count[3]);
+  const int above = sm.count[3];
+  if (above <= CAP) {
+    rank_keys<THREADS>(sm.cand, above, sm.best);
+    int have = above;                                 // those equal to the bound follow in index order
+    for (int base = lo; base < hi && have < k; base += THREADS) {
+      const int i = base + tid;
+      const bool eq = i < hi && value_key(to_f(r[i])) == bound;
+      const uint32_t votes = __ballot_sync(0xffffffffu, eq);
+      __syncthreads();
+      if (lane == 0) sm.groups[warp] = __popc(votes);
+      __syncthreads();
+      int before = have, all = have;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += sm.groups[w];
+        all += sm.groups[w];
+      }
+      const int at = before + __popc(votes & ((1u << lane) - 1));
+      if (eq && at < 32) sm.best[at] = order_key(to_f(r[i]), i);
+      have = all;
+    }
+    __syncthreads();
+    return;
+  }
+  unsigned long long last = ~0ull;
   for (int c = 0; c < k; ++c) {
     unsigned long long b = 0;
     for (int i = lo + tid; i < hi; i += THREADS) {
@@ -280,21 +291,22 @@ __device__ __noinline__ unsigned long long part_top(const T* r, int first_vec, i
     __syncthreads();
     for (int w = 0; w < WARPS; ++w) b = sm.cand[w] > b ? sm.cand[w] : b;
     last = b;
-    if (lane == c) mine = b;
+    if (tid == 0) sm.best[c] = b;
   }
-  return mine;
+  __syncthreads();
 }
 
 // One read of the logits: a row, or a part of it where there are few rows (the CTAs of a cluster then leave their sums and
 // alternatives with the first one). Every thread keeps a running maximum and sums relative to it, and the maxima of its chunks
 // for the alternatives.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS)
 logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
                 long long ignore_index, int parts, float* __restrict__ logprob, float* __restrict__ entropy,
                 float2* __restrict__ stats, float* __restrict__ top_lp, long long* __restrict__ top) {
-  constexpr int L = Vec<T>::L;
-  __shared__ Smem sm;
+  constexpr int L = Vec<T>::L, WARPS = THREADS / 32;
+  __shared__ SumsSmem<THREADS> sm;
+  __shared__ typename std::conditional<TOP, TopSmem<THREADS>, int>::type ts;
   const long long row = blockIdx.x / parts;
   const int part = static_cast<int>(blockIdx.x % parts);
   const T* r = x + row * ld;
@@ -330,10 +342,8 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   auto take = [&](const uint4& v) {
     float f[L];
     Vec<T>::unpack(v, f);
-    float vm = f[0];
-#pragma unroll
-    for (int j = 1; j < L; ++j) vm = max_nan(vm, f[j]);
-    cmax = max_nan(cmax, vm);
+    const float vm = Vec<T>::largest(v);
+    if (TOP) cmax = max_nan(cmax, vm);
     if (vm > a.m) a.raise(vm, c);
     const float mo = -a.m * c;
 #pragma unroll
@@ -352,18 +362,18 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     for (int q = 0; q < 4; ++q) v[q] = i + q * THREADS < end_vec ? load_stream(g + i + q * THREADS) : none;
 #pragma unroll
     for (int q = 0; q < 4; ++q) take(v[q]);
-    if (TOP) {
+    if constexpr (TOP) {
       in_chunk += 4;
       if (in_chunk == cl) {
-        sm.cmax[chunk++][tid] = cmax;
+        ts.cmax[chunk++][tid] = cmax;
         tmax = max_nan(tmax, cmax);
         cmax = -INFINITY;
         in_chunk = 0;
       }
     }
   }
-  if (TOP) {
-    if (in_chunk) sm.cmax[chunk][tid] = cmax;
+  if constexpr (TOP) {
+    if (in_chunk) ts.cmax[chunk][tid] = cmax;
     tmax = max_nan(tmax, cmax);
   }
   // the elements before and after the vectors, one a thread
@@ -379,14 +389,40 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     a.s += e;
     a.u = fmaf(d, e, a.u);
   }
-  const float m = block_reduce(a.m, sm.red, [](float p, float q) { return fmaxf(p, q); });
-  a.raise(m, c);
-  auto add = [](float p, float q) { return p + q; };
-  Sums all{m, block_reduce(a.s, sm.red, add), block_reduce(a.u, sm.red, add)};
-  unsigned long long best = 0;
+  // the sums of the warp, then of the block: in the same order in every thread
+  float wm = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+  a.raise(wm, c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  if (lane == 0) {
+    sm.warp[tid >> 5][0] = wm;
+    sm.warp[tid >> 5][1] = a.s;
+    sm.warp[tid >> 5][2] = a.u;
+  }
+  __syncthreads();
+  auto combine = [&](const float (*of)[3], int n) {
+    float top_m = of[0][0];
+#pragma unroll 4
+    for (int i = 1; i < n; ++i) top_m = fmaxf(top_m, of[i][0]);
+    Sums t{top_m, 0.f, 0.f};
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+      Sums o{of[i][0], of[i][1], of[i][2]};
+      o.raise(top_m, c);
+      t.s += o.s;
+      t.u += o.u;
+    }
+    return t;
+  };
+  Sums all = combine(sm.warp, WARPS);
   if constexpr (TOP) {
     const int lo = part == 0 ? 0 : span.head + first_vec * L, hi = part == parts - 1 ? V : span.head + end_vec * L;
-    best = part_top(r, first_vec, end_vec, span.head, edge, edge_at, tmax, cl, k, lo, hi, sm);
+    part_top<T, THREADS>(r, first_vec, end_vec, span.head, edge, edge_at, tmax, cl, k, lo, hi, ts);
   }
   if (parts > 1) {
     cluster_wait();                                  // every CTA of the cluster has started: the first one's memory is there
@@ -397,28 +433,26 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(all.s) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(all.u) : "memory");
       }
-      if (TOP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_cta(smem_u32(&sm.lists[part][lane]), 0)), "l"(best) : "memory");
+      if constexpr (TOP)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_cta(smem_u32(&ts.lists[part * 32 + lane]), 0)), "l"(ts.best[lane]) : "memory");
     }
     __syncwarp();
     cluster_sync_all();
     if (part != 0) return;
-    float top_m = sm.part[0][0];
-    for (int p = 1; p < parts; ++p) top_m = fmaxf(top_m, sm.part[p][0]);
-    all = Sums{top_m, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-      Sums o{sm.part[p][0], sm.part[p][1], sm.part[p][2]};
-      o.raise(top_m, c);
-      all.s += o.s;
-      all.u += o.u;
+    all = combine(sm.part, parts);
+    if constexpr (TOP) {
+      if (tid < 32) ts.best[tid] = 0;
+      __syncthreads();
+      rank_keys<THREADS>(ts.lists, parts * 32, ts.best);
+      __syncthreads();
     }
-    if (TOP && tid < 32)
-      for (int p = 1; p < parts; ++p) best = warp_merge(best, sm.lists[p][31 - lane], lane);
   }
   float log_s = logf(all.s), H = log_s - all.u * LN2 / all.s;
   if (!(all.m > floor_ && fabsf(all.m * c) < 1e38f && fabsf(all.s) < INFINITY)) {      // the same in all threads
+    auto add = [](float p, float q) { return p + q; };
     float mx = -INFINITY;
     for (int i = tid; i < V; i += THREADS) mx = max_nan(mx, to_f(r[i]));
-    mx = block_reduce(mx, sm.red, [](float p, float q) { return max_nan(p, q); });
+    mx = block_reduce<THREADS>(mx, sm.red, [](float p, float q) { return max_nan(p, q); });
     float s = 0.f, u = 0.f;
     for (int i = tid; i < V; i += THREADS) {
       const float d = (to_f(r[i]) - mx) * inv_t;
@@ -428,8 +462,8 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
         u += e == 0.f ? 0.f : d * e;
       }
     }
-    s = block_reduce(s, sm.red, add);
-    u = block_reduce(u, sm.red, add);
+    s = block_reduce<THREADS>(s, sm.red, add);
+    u = block_reduce<THREADS>(u, sm.red, add);
     all.m = mx;
     log_s = logf(s);
     H = log_s - u / s;
@@ -439,19 +473,20 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     entropy[row] = H;
     stats[row] = make_float2(all.m, log_s);
   }
-  if (TOP && tid < k) {
-    const int at = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
-    const uint32_t key = static_cast<uint32_t>(best >> 32);
-    const float v = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-    top[row * k + tid] = at;
-    top_lp[row * k + tid] = (v - all.m) * inv_t - log_s;
+  if constexpr (TOP) {
+    if (tid < k) {
+      const unsigned long long best = ts.best[tid];
+      const float v = key_value(static_cast<uint32_t>(best >> 32));
+      top[row * k + tid] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+      top_lp[row * k + tid] = (v - all.m) * inv_t - log_s;
+    }
   }
 }
 
 // dx_j = [ -p_j (G + gH (log p_j + H)) + g [j = target] + sum_i g_i [j = top_i] ] / temperature, G = g + sum_i g_i.
 // Row blockIdx.x, part blockIdx.y. With l = log2 p_j the first term is p_j (l A + B); the chosen positions are written again.
-template <typename T>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS)
 logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
                     long long ignore_index, const long long* __restrict__ top, const float2* __restrict__ stats,
                     const float* __restrict__ entropy, const float* __restrict__ glp, const float* __restrict__ gh,
@@ -539,6 +574,8 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ targe
   }
 }
 
+constexpr int SMALL_V = 8192, LARGE = 256;
+
 // CTAs of a row: enough to fill the SMs twice, but at least 4096 elements each.
 int row_parts(long long T, int V) {
   int parts = 1;
@@ -561,7 +598,8 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
   if (T * parts > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(T * parts), 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  const bool small = V <= SMALL_V;
+  cfg.blockDim = dim3(small ? 128 : LARGE, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -572,7 +610,8 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
   cfg.numAttrs = parts > 1 ? 1 : 0;
   auto run = [&](auto* p) {
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    auto kernel = k > 0 ? logprobs_kernel<E, true> : logprobs_kernel<E, false>;
+    auto kernel = k > 0 ? (small ? logprobs_kernel<E, true, 128> : logprobs_kernel<E, true, LARGE>)
+                        : (small ? logprobs_kernel<E, false, 128> : logprobs_kernel<E, false, LARGE>);
     const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p, target, V, ld, inv_t, k, ignore_index, parts, logprob, entropy,
                                                static_cast<float2*>(stats), top_lp, top);
     const int rc = ok();   // also clears the error of a launch that failed
@@ -594,8 +633,10 @@ FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* tar
   auto run = [&](auto* p) {
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
     const dim3 grid(static_cast<unsigned>(T), row_parts(T, V));
-    logprobs_bwd_kernel<<<grid, THREADS, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
-                                                                          static_cast<const float2*>(stats), entropy, glp, gh, gtop, static_cast<E*>(dx), ldd);
+    auto kernel = V <= SMALL_V ? logprobs_bwd_kernel<E, 128> : logprobs_bwd_kernel<E, LARGE>;
+    kernel<<<grid, V <= SMALL_V ? 128 : LARGE, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
+                                                            static_cast<const float2*>(stats), entropy, glp, gh, gtop,
+                                                            static_cast<E*>(dx), ldd);
     return ok();
   };
   if (kind == 0) return run(static_cast<const __nv_bfloat16*>(x));
