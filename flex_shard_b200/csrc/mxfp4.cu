@@ -343,6 +343,235 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   }
 }
 
+// ------------------------------------------------------------------ block-scaled product on SM pairs
+// 256 x 256 tiles of a CTA pair, rows t as the M operand. Per CTA and stage: 128 rows of each operand, the scale blocks of its
+// own 128 rows of A (two: 1 KB) and of all 256 rows of B (four), which the tensor core of each SM wants in its own TMEM;
+// tcgen05.cp on a pair copies them in both CTAs at once. An accumulator of 256 columns and the scales leave no room for a
+// second one, so eight warps move a finished tile from TMEM into registers and hand the accumulator back before they store it.
+constexpr int P_BN = 256;
+constexpr int P_A = BM * KB, P_B = BM * KB;
+constexpr int P_STAGE_BYTES = P_A + P_B + 3 * SF_BYTES;   // 35 KB
+constexpr int P_STAGES = 6;
+constexpr int P_SMEM = P_STAGES * P_STAGE_BYTES + 1024 + 256;
+constexpr int P_THREADS = 64 + 32 * 8;   // warp 0 TMA, warp 1 MMA, warps 2..9 epilogue (two per lane quarter, 128 columns each)
+constexpr int P_SF_COL0 = 256, P_SF_SET = 32;   // a stage's scales: 2 x 4 columns of A, 2 x 8 of B
+
+__device__ __forceinline__ void tmem_cp_32x128b_x4_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tsfa,
+                                               uint32_t tsfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tsfa), "r"(tsfb)
+      : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb, const Args args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P_STAGES * P_STAGE_BYTES);
+  uint64_t* full_bar = bars;                        // [P_STAGES]  used in CTA 0
+  uint64_t* empty_bar = bars + P_STAGES;            // [P_STAGES]  one per CTA
+  uint64_t* tmem_full = bars + 2 * P_STAGES;        // one per CTA
+  uint64_t* tmem_empty = bars + 2 * P_STAGES + 1;   // used in CTA 0: the epilogue warps of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * P_STAGES + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int tiles_m = (args.M + 2 * BM - 1) / (2 * BM), tiles_n = (args.N + P_BN - 1) / P_BN;
+  const int num_tiles = tiles_m * tiles_n;
+  const int num_kb = (args.K + BK - 1) / BK;
+  const int tile0 = static_cast<int>(blockIdx.x >> 1), tile_step = static_cast<int>(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(tmem_full, 1);
+    mbar_init(tmem_empty, 16);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // the peer's barriers are initialised before anything is signalled across the pair
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&map_a);
+      tma_prefetch_desc(&map_b);
+      tma_prefetch_desc(&map_sfa);
+      tma_prefetch_desc(&map_sfb);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = tile0; tile < num_tiles && ok; tile += tile_step) {
+        int tm, tn;
+        grouped_tile_coords(tile, tiles_m, tiles_n, tm, tn);
+        const int mb = tm * 2 + static_cast<int>(rank);   // 128-row block of A
+        const int m0 = mb * BM, n0 = tn * P_BN + static_cast<int>(rank) * BM;
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const int s = it % P_STAGES;
+          if (!mbar_wait(&empty_bar[s], ((it / P_STAGES) & 1) ^ 1, abort_flag)) {
+            atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_EMPTY);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + s * P_STAGE_BYTES;
+          uint8_t* sb = sa + P_A;
+          uint8_t* ssf = sb + P_B;
+          const uint32_t full0 = map_to_cta(smem_u32(&full_bar[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * P_STAGE_BYTES);   // the bytes of both CTAs
+          tma_load_2d_pair(sa, &map_a, full0, kb * KB, m0);
+          tma_load_2d_pair(sb, &map_b, full0, kb * KB, n0);
+          // blocks past the last one read as zeros, like the codes they belong to
+          tma_load_2d_pair(ssf, &map_sfa, full0, kb * 256, mb);
+          tma_load_2d_pair(ssf + SF_BYTES, &map_sfb, full0, kb * 256, tn * 2);   // two rows of blocks
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {   // one CTA issues for the pair; the whole warp walks the loop
+      uint32_t it = 0, local_tile = 0;
+      bool ok = true;
+      for (int tile = tile0; tile < num_tiles && ok; tile += tile_step, ++local_tile) {
+        if (!mbar_wait(tmem_empty, (local_tile & 1) ^ 1, abort_flag)) {
+          if (lane == 0) {
+            atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_TMEM_EMPTY);
+            *abort_flag = 1;
+          }
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const int s = it % P_STAGES;
+          if (!mbar_wait(&full_bar[s], (it / P_STAGES) & 1, abort_flag)) {
+            if (lane == 0) {
+              atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_FULL);
+              *abort_flag = 1;
+            }
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * P_STAGE_BYTES);
+          const uint64_t da = make_smem_desc_sw128(sa, 16, 1024);
+          const uint64_t db = make_smem_desc_sw128(sa + P_A, 16, 1024);
+          const uint32_t ssf = sa + P_A + P_B;
+          const uint32_t tsfa = tmem_base + P_SF_COL0 + (it & 1) * P_SF_SET, tsfb = tsfa + 8;
+          const uint32_t e_own = smem_u32(&empty_bar[s]);
+          if (elect_one()) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {   // the two 128-deep halves of the stage
+              tmem_cp_32x128b_x4_pair(tsfa + 4 * h, make_sf_desc(ssf + 512 * h));
+              tmem_cp_32x128b_x4_pair(tsfb + 8 * h, make_sf_desc(ssf + SF_BYTES + 512 * h));
+              tmem_cp_32x128b_x4_pair(tsfb + 8 * h + 4, make_sf_desc(ssf + 2 * SF_BYTES + 512 * h));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_mxf4_pair(tmem_base, da + 2 * k, db + 2 * k, make_idesc_mx4(2 * BM, P_BN, (k & 1) * 2), tsfa + 4 * (k >> 1),
+                             tsfb + 8 * (k >> 1), (kb | k) != 0);
+            umma_commit_pair(e_own);
+            umma_commit_pair(map_to_cta(e_own, 1));
+          }
+          __syncwarp();
+        }
+        if (ok) {
+          const uint32_t f_own = smem_u32(tmem_full);
+          if (elect_one()) {
+            umma_commit_pair(f_own);
+            umma_commit_pair(map_to_cta(f_own, 1));
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int part = (warp - 2) >> 2;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + part * 128;
+    uint32_t local_tile = 0;
+    for (int tile = tile0; tile < num_tiles; tile += tile_step, ++local_tile) {
+      int tm, tn;
+      grouped_tile_coords(tile, tiles_m, tiles_n, tm, tn);
+      const int row = (tm * 2 + static_cast<int>(rank)) * BM + quarter * 32 + lane;
+      if (!mbar_wait_warp(tmem_full, local_tile & 1, abort_flag)) {
+        if (lane == 0) {
+          atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_TMEM_FULL);
+          *abort_flag = 1;
+        }
+        break;
+      }
+      tc_fence_after();
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_row + 32 * c, v[c]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(tmem_empty), 0));   // the next tile may start
+      if (row >= args.M) continue;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int col = tn * P_BN + part * 128 + c * 32;
+        const int ncols = min(32, args.N - col);
+        if (args.d_fp32) {
+          float* dp = static_cast<float*>(args.d) + static_cast<long long>(row) * args.ldd + col;
+          if (ncols == 32 && (reinterpret_cast<uintptr_t>(dp) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dp + i) = make_uint4(v[c][i], v[c][i + 1], v[c][i + 2], v[c][i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < ncols) dp[i] = __uint_as_float(v[c][i]);
+          }
+        } else {
+          __nv_bfloat16* dp = static_cast<__nv_bfloat16*>(args.d) + static_cast<long long>(row) * args.ldd + col;
+          if (ncols == 32 && (reinterpret_cast<uintptr_t>(dp) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 o;
+              o.x = pack_bf16x2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+              o.y = pack_bf16x2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3]));
+              o.z = pack_bf16x2(__uint_as_float(v[c][i + 4]), __uint_as_float(v[c][i + 5]));
+              o.w = pack_bf16x2(__uint_as_float(v[c][i + 6]), __uint_as_float(v[c][i + 7]));
+              *reinterpret_cast<uint4*>(dp + i) = o;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < ncols) dp[i] = __float2bfloat16(__uint_as_float(v[c][i]));
+          }
+        }
+      }
+    }
+  }
+
+  // Every loop above is bounded, so all warps of both CTAs arrive here; neither CTA may leave before both are done.
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    if (*abort_flag) {
+      const unsigned long long t0 = clock64();
+      while (clock64() - t0 < 2000000ull) {
+      }
+    }
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH; }
 
 // codes [rows, K] as bytes, boxes of box_rows rows x 128 bytes
@@ -376,6 +605,28 @@ int launch(const void* aq, const void* sfa, const void* bq, const void* sfb, con
   const dim3 grid((a.N + BM - 1) / BM, (a.M + BN - 1) / BN);
   if (grid.y > 65535) return FSB_ERR_TOO_LARGE;
   gemm_mxfp4_kernel<BN><<<grid, NUM_THREADS, Tile<BN>::SMEM, stream>>>(map_w, map_x, map_sfw, map_sfx, a);
+  return ok();
+}
+
+// Clusters of the pair kernel that fit the current device at once (-1: unusable).
+int resident_pairs() {
+  static int pairs[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return -1;
+  if (pairs[dev] == 0) pairs[dev] = fsb_resident_pairs(gemm_mxfp4_pair_kernel, P_THREADS, P_SMEM);
+  return pairs[dev];
+}
+int launch_pairs(const void* aq, const void* sfa, const void* bq, const void* sfb, const Args& a, long long lda, long long ldb,
+                 int pairs, cudaStream_t stream) {
+  CUtensorMap map_a, map_b, map_sfa, map_sfb;
+  int rc = codes_map(&map_a, aq, a.M, a.K, lda, BM);
+  if (rc == FSB_OK) rc = codes_map(&map_b, bq, a.N, a.K, ldb, BM);
+  if (rc == FSB_OK) rc = scales_map(&map_sfa, sfa, a.M, a.K, 1);
+  if (rc == FSB_OK) rc = scales_map(&map_sfb, sfb, a.N, a.K, 2);
+  if (rc != FSB_OK) return rc;
+  const int tiles = ((a.M + 2 * BM - 1) / (2 * BM)) * ((a.N + P_BN - 1) / P_BN);
+  gemm_mxfp4_pair_kernel<<<2 * (tiles < pairs ? tiles : pairs), P_THREADS, P_SMEM, stream>>>(map_a, map_b, map_sfa, map_sfb, a);
   return ok();
 }
 }  // namespace
@@ -437,5 +688,9 @@ FSB_API int fsb_gemm_mxfp4(const void* aq, const void* sfa, const void* bq, cons
   if (M <= 16) return launch<16>(aq, sfa, bq, sfb, a, lda, ldb, stream);
   if (M <= 32) return launch<32>(aq, sfa, bq, sfb, a, lda, ldb, stream);
   if (M <= 64) return launch<64>(aq, sfa, bq, sfb, a, lda, ldb, stream);
+  if (M > 512) {
+    const int pairs = resident_pairs();
+    if (pairs > 0) return launch_pairs(aq, sfa, bq, sfb, a, lda, ldb, pairs, stream);
+  }
   return launch<128>(aq, sfa, bq, sfb, a, lda, ldb, stream);
 }

@@ -56,7 +56,8 @@ def check_product(y, a, b):
 
 @pytest.mark.parametrize("M,N,K", [
     (1, 128, 256), (1, 1, 32), (1, 4096, 4096), (3, 130, 96), (16, 256, 160), (17, 384, 1024), (32, 100, 2080), (48, 1000, 512),
-    (64, 129, 4096), (65, 128, 128), (128, 512, 1152), (129, 300, 640), (257, 1000, 800), (777, 1290, 416), (1024, 2048, 256)])
+    (64, 129, 4096), (65, 128, 128), (128, 512, 1152), (129, 300, 640), (257, 1000, 800), (777, 1290, 416), (1024, 2048, 256), (513, 257, 32), (600, 3000, 1056),
+    (2305, 2440, 288), (4104, 1560, 384), (1300, 9000, 4096)])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_product(M, N, K, dt):
     aq, sa, a = operand(M, K, 1)
