@@ -58,102 +58,166 @@ __device__ __forceinline__ uint4 load8_any(const __nv_bfloat16* p, bool vec) {
 }
 
 // ------------------------------------------------------------------ activation quantiser (1x32 groups)
-// Four threads per group, 8 columns each. Rows past T and groups past K / 32 get the scale byte 127.
+// Two threads per group, 16 columns each, UNITS such pieces a thread in flight: bound by memory, 2.53 bytes an element. The
+// eight threads of a scale block's row gather its four bytes into one word. Rows past T and groups past K / 32 get the byte
+// 127. I: the type that counts pieces (a 64-bit quotient per piece costs as much as the rest).
+// 5765 x 14336: 40.9 us (5.1 TB/s); one piece a thread 43.9, four 42.6; with 64-bit counting and 8 columns a thread 67.9.
+constexpr int UNITS = 2;
+template <typename I>
 __global__ void __launch_bounds__(256)
 mx4_quant_act_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scales, long long T,
                      int K, long long ldx, int n_gb, int vec) {
-  const int units = n_gb * 16;                        // threads of a padded row
-  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-  const long long row = i / units;
-  const int u = static_cast<int>(i - row * units);
-  if (row >= (T + 127) / 128 * 128) return;           // the four threads of a group leave together
-  const bool live = row < T && u * 8 < K;
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (live) v = load8_any(x + row * ldx + u * 8, vec);
-  uint32_t m = amax8_bits(v, 0u);
-  const unsigned group = 0xfu << (threadIdx.x & 28);
-  m = max(m, __shfl_xor_sync(group, m, 2));
-  m = max(m, __shfl_xor_sync(group, m, 1));
-  const uint32_t e = mx4_exponent(m);
-  if ((u & 3) == 0) scales[blocked_offset(row, u >> 2, n_gb)] = live ? static_cast<uint8_t>(e) : 127;
-  if (live) *reinterpret_cast<uint32_t*>(q + row * (K / 2) + u * 4) = quant8_fp4(v, mx4_inv(e));
+  const I units = n_gb * 8;                               // pieces of a padded row
+  const I total = static_cast<I>((T + 127) / 128 * 128) * units, share = total / UNITS;   // both multiples of 8
+  const I i0 = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i0 >= share) return;                                // the eight threads of a row's block leave together
+  uint4 v[UNITS][2];
+  long long row[UNITS];
+  int u[UNITS];
+  bool live[UNITS];
+#pragma unroll
+  for (int j = 0; j < UNITS; ++j) {
+    const I i = i0 + j * share, r = i / units;
+    row[j] = r;
+    u[j] = static_cast<int>(i - r * units);
+    live[j] = row[j] < T && u[j] * 16 < K;
+    v[j][0] = v[j][1] = make_uint4(0, 0, 0, 0);
+    if (live[j]) {
+      const __nv_bfloat16* p = x + row[j] * ldx + u[j] * 16;
+      v[j][0] = load8_any(p, vec);
+      v[j][1] = load8_any(p + 8, vec);
+    }
+  }
+  const unsigned octet = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+  for (int j = 0; j < UNITS; ++j) {
+    uint32_t m = amax8_bits(v[j][1], amax8_bits(v[j][0], 0u));
+    m = max(m, __shfl_xor_sync(octet, m, 1));
+    const uint32_t e = mx4_exponent(m);
+    uint32_t word = (live[j] ? e : 127u) << (4 * (threadIdx.x & 6));
+    word |= __shfl_xor_sync(octet, word, 2);
+    word |= __shfl_xor_sync(octet, word, 4);
+    if ((threadIdx.x & 7) == 0) *reinterpret_cast<uint32_t*>(scales + blocked_offset(row[j], u[j] >> 1, n_gb)) = word;
+    if (live[j]) {
+      const float inv = mx4_inv(e);
+      *reinterpret_cast<uint2*>(q + row[j] * (K / 2) + u[j] * 8) = make_uint2(quant8_fp4(v[j][0], inv), quant8_fp4(v[j][1], inv));
+    }
+  }
 }
 
 // ------------------------------------------------------------------ weight quantiser (32x32 tiles)
-// A warp per tile: lane l holds 8 columns of rows l/4, l/4 + 8, l/4 + 16, l/4 + 24. One tile exponent serves the forward
-// product (groups along the columns) and the input gradient (groups along the rows). Besides the tile exponents it can write
-// the blocked scales of both operands: tiles past the edges, up to whole 128 x 128 blocks, write the padding.
+// A block takes 128 rows x 32 TC columns, a warp 32 rows of them: TC tiles, 4 TC 16-byte reads a lane in flight, 64 TC bytes of a
+// row side by side. One tile exponent serves the forward product (groups along the columns) and the input gradient (groups along
+// the rows); the block writes its part of the scale block of either operand, padding included (a grid that covers whole scale
+// blocks). Bound by memory, 2.53 bytes an element: 28660 x 4096 58.6 us (5.1 TB/s) with TC = 4, 60.2 with TC = 1, which gives a
+// small weight four times the blocks: 500 x 2048 2.7 us against 4.5.
+template <int TC>
 __global__ void __launch_bounds__(128)
 mx4_quant_weight_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __restrict__ q, uint8_t* __restrict__ tile_exp,
                         uint8_t* __restrict__ fwd, uint8_t* __restrict__ dgrad, int rows, int cols, long long ldw, int vec) {
-  const int tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int exp_rows = (rows + 31) / 32, exp_cols = cols / 32, rt = blockIdx.y;
-  const bool inside = rt < exp_rows && tile < exp_cols;
-  uint32_t e = 127;
-  if (inside) {
-    const int r0 = rt * 32 + (lane >> 2), c0 = tile * 32 + (lane & 3) * 8;
-    uint4 v[4];
-    uint32_t m = 0;
+  constexpr int LANES = 4 * TC, STEP = 32 / LANES;    // lanes of a row, rows of a pass
+  __shared__ uint8_t exps[4][TC];                     // [tile row][tile column] of the block; 127 outside the matrix
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x * 32 * TC + lane % LANES * 8;
+  const long long row0 = static_cast<long long>(blockIdx.y) * 128 + warp * 32, r0 = row0 + lane / LANES;
+  const bool in_cols = c0 < cols;
+  uint4 v[LANES];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + 8 * i;
-      v[i] = r < rows ? load8_any(w + r * ldw + c0, vec) : make_uint4(0, 0, 0, 0);
-    }
+  for (int i = 0; i < LANES; ++i)
+    v[i] = in_cols && r0 + STEP * i < rows ? load8_any(w + (r0 + STEP * i) * ldw + c0, vec) : make_uint4(0, 0, 0, 0);
+  uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = amax8_bits(v[i], m);
-    m = __reduce_max_sync(0xffffffffu, m);
-    e = mx4_exponent(m);
-    if (lane == 0) tile_exp[static_cast<long long>(rt) * exp_cols + tile] = static_cast<uint8_t>(e);
-    const float inv = mx4_inv(e);
+  for (int i = 0; i < LANES; ++i) m = amax8_bits(v[i], m);
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + 8 * i;
-      if (r < rows) *reinterpret_cast<uint32_t*>(q + static_cast<long long>(r) * (cols / 2) + c0 / 2) = quant8_fp4(v[i], inv);
-    }
+  for (int o = LANES; o < 32; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const uint32_t e = mx4_exponent(m);
+  const float inv = mx4_inv(e);
+#pragma unroll
+  for (int i = 0; i < LANES; ++i)
+    if (in_cols && r0 + STEP * i < rows) *reinterpret_cast<uint32_t*>(q + (r0 + STEP * i) * (cols / 2) + c0 / 2) = quant8_fp4(v[i], inv);
+  if (lane < LANES && (lane & 3) == 0) {
+    const bool inside = in_cols && row0 < rows;
+    exps[warp][lane >> 2] = inside ? static_cast<uint8_t>(e) : 127;
+    if (inside) tile_exp[(row0 >> 5) * (cols / 32) + (c0 >> 5)] = static_cast<uint8_t>(e);
   }
-  const int col_blocks = (cols + 127) / 128, row_blocks = (rows + 127) / 128;
-  if (fwd != nullptr) {
-    const long long r = static_cast<long long>(rt) * 32 + lane;
-    fwd[blocked_offset(r, tile, col_blocks)] = static_cast<uint8_t>(r < rows ? e : 127);
+  if (fwd == nullptr) return;
+  __syncthreads();
+  const int t = threadIdx.x, col_blocks = (cols + 127) / 128;
+  const long long at = static_cast<long long>(blockIdx.y) * 128 + t;            // row of the forward operand
+#pragma unroll
+  for (int g = 0; g < TC; ++g) fwd[blocked_offset(at, blockIdx.x * TC + g, col_blocks)] = at < rows ? exps[t >> 5][g] : 127;
+  if (t < 32 * TC) {                                                            // row of the transposed operand: four groups
+    uint32_t d = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) d |= static_cast<uint32_t>(exps[g][t >> 5]) << (8 * g);
+    *reinterpret_cast<uint32_t*>(dgrad + blocked_offset(static_cast<long long>(blockIdx.x) * 32 * TC + t, blockIdx.y * 4, gridDim.y)) = d;
   }
-  if (dgrad != nullptr) dgrad[blocked_offset(static_cast<long long>(tile) * 32 + lane, rt, row_blocks)] = static_cast<uint8_t>(e);
 }
 
 // ------------------------------------------------------------------ expansion
-// Codes as the values they stand for: e4m3 without the scales (kind 0, every e2m1 value is one of e4m3), bf16 (1) or fp32 (2)
-// with them. e2m1 values times powers of two are exact in all three, but for what underflows. Eight codes a thread.
+// Codes as the values they stand for: e4m3 without the scales (KIND 0, every e2m1 value is one of e4m3), bf16 (1) or fp32 (2)
+// with them. e2m1 values times powers of two are exact in all three, but for what underflows. Pieces of 16 (e4m3) or 8 codes,
+// EXPAND_UNITS a thread in flight: bound by memory. 28660 x 4096 to bf16 / e4m3: 50 / 29 us (5.9 / 6.1 TB/s), two pieces a thread
+// 55 / 30, one 68 / 35.
+constexpr int EXPAND_UNITS = 4;
+__device__ __forceinline__ __half2 fp4x2_values(uint32_t byte) {
+  return __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1));
+}
+template <int KIND, typename I>
 __global__ void __launch_bounds__(256)
 mx4_expand_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, void* __restrict__ out, long long T, int K,
-                  long long ldq, int n_gb, int kind) {
-  const int units = K / 8;
-  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-  const long long row = i / units;
-  if (row >= T) return;
-  const int u = static_cast<int>(i - row * units);
-  const uint32_t c = *reinterpret_cast<const uint32_t*>(q + row * ldq + u * 4);
-  const float s = kind == 0 ? 1.f : mx4_scale(scales[blocked_offset(row, u >> 2, n_gb)]);
-  float f[8];
+                  long long ldq, int n_gb) {
+  constexpr int C = KIND == 0 ? 16 : 8;
+  const I units = K / C, total = static_cast<I>(T) * units, share = (total + EXPAND_UNITS - 1) / EXPAND_UNITS;
+  const I i0 = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i0 >= share) return;
+  uint32_t c[EXPAND_UNITS][C / 8];
+  uint32_t e[EXPAND_UNITS];
+  long long at[EXPAND_UNITS];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t code = c >> (4 * j), mag = code & 7u;
-    // magnitudes 0, .5, then (1 + mantissa / 2) 2^(exponent - 1)
-    const float a = mag < 2 ? 0.5f * mag : __uint_as_float((126u + (mag >> 1)) << 23 | (mag & 1u) << 22);
-    f[j] = (code & 8u ? -a : a) * s;
+  for (int j = 0; j < EXPAND_UNITS; ++j) {
+    const I i = i0 + j * share, r = i / units;
+    const int u = static_cast<int>(i - r * units);
+    at[j] = i < total ? static_cast<long long>(r) * K + u * C : -1;
+    if (at[j] < 0) continue;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(q + static_cast<long long>(r) * ldq) + u * (C / 8);
+#pragma unroll
+    for (int w = 0; w < C / 8; ++w) c[j][w] = p[w];
+    if (KIND != 0) e[j] = scales[blocked_offset(r, u >> 2, n_gb)];
   }
-  const long long at = row * K + u * 8;
-  if (kind == 2) {
-    float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-    d[0] = make_float4(f[0], f[1], f[2], f[3]);
-    d[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else if (kind == 1) {
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at) =
-        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  } else {
-    uint2 o;
-    uint16_t* h = reinterpret_cast<uint16_t*>(&o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * j], f[2 * j + 1]), __NV_SATFINITE, __NV_E4M3);
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(out) + at) = o;
+  for (int j = 0; j < EXPAND_UNITS; ++j) {
+    if (at[j] < 0) continue;
+    if constexpr (KIND == 0) {
+      uint32_t o[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t two = c[j][w >> 1] >> (16 * (w & 1));
+        const uint32_t lo = __nv_cvt_halfraw2_to_fp8x2(fp4x2_values(two & 0xffu), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_halfraw2_to_fp8x2(fp4x2_values(two >> 8 & 0xffu), __NV_SATFINITE, __NV_E4M3);
+        o[w] = lo | hi << 16;
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + at[j]) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+      const float s = mx4_scale(e[j]);
+      float2 f[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        f[w] = __half22float2(fp4x2_values(c[j][0] >> (8 * w) & 0xffu));
+        f[w].x *= s;
+        f[w].y *= s;
+      }
+      if constexpr (KIND == 2) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at[j]);
+        d[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+        d[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at[j]) =
+            make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y), pack_bf16x2(f[3].x, f[3].y));
+      }
+    }
   }
 }
 
@@ -633,29 +697,36 @@ int launch_pairs(const void* aq, const void* sfa, const void* bq, const void* sf
 
 // x: bf16 [T, K], K % 32 == 0, row stride ldx; q: [T, K / 2] bytes; scales: pad128(T) * pad4(K / 32) bytes, all written.
 FSB_API int fsb_mx4_quant_act(const void* x, void* q, void* scales, long long T, int K, long long ldx, cudaStream_t stream) {
-  if (K <= 0 || K % 32 != 0 || T < 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0) return FSB_ERR_BAD_ARG;
+  if (K <= 0 || K % 32 != 0 || T < 0 || (reinterpret_cast<uintptr_t>(q) & 7) != 0 || (reinterpret_cast<uintptr_t>(scales) & 3) != 0)
+    return FSB_ERR_BAD_ARG;
   if (T == 0) return FSB_OK;
   const int n_gb = (K + 127) / 128;
-  const long long blocks = ((T + 127) / 128 * 128 * (n_gb * 16) + 255) / 256;
+  const long long share = (T + 127) / 128 * 128 * (n_gb * 8) / UNITS, blocks = (share + 255) / 256;
   if (blocks > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx % 8 == 0;
-  mx4_quant_act_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-      static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales), T, K, ldx, n_gb, vec);
+  auto kernel = share * UNITS < (1ll << 31) ? mx4_quant_act_kernel<unsigned> : mx4_quant_act_kernel<long long>;
+  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q),
+                                                            static_cast<uint8_t*>(scales), T, K, ldx, n_gb, vec);
   return ok();
 }
 
-// w: bf16 [rows, cols], cols % 32 == 0; q: [rows, cols / 2] bytes; tile_exp: [ceil(rows / 32), cols / 32] bytes. fwd / dgrad
-// (each may be null): blocked scales of the operands [rows, cols] and [cols, rows], padding included.
+// w: bf16 [rows, cols], cols % 32 == 0; q: [rows, cols / 2] bytes; tile_exp: [ceil(rows / 32), cols / 32] bytes. fwd / dgrad:
+// blocked scales of the operands [rows, cols] and [cols, rows], padding included (both or neither).
 FSB_API int fsb_mx4_quant_weight(const void* w, void* q, void* tile_exp, void* fwd, void* dgrad, int rows, int cols, long long ldw,
                                  cudaStream_t stream) {
-  if (rows < 0 || cols <= 0 || cols % 32 != 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0) return FSB_ERR_BAD_ARG;
+  if (rows < 0 || cols <= 0 || cols % 32 != 0 || (fwd == nullptr) != (dgrad == nullptr) ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(fwd) | reinterpret_cast<uintptr_t>(dgrad)) & 3) != 0)
+    return FSB_ERR_BAD_ARG;
   if (rows == 0) return FSB_OK;
-  const dim3 grid((cols + 127) / 128, (rows + 127) / 128 * 4);
-  if (grid.y > 65535) return FSB_ERR_TOO_LARGE;
+  const int col_blocks = (cols + 127) / 128;
+  const long long row_blocks = (static_cast<long long>(rows) + 127) / 128;
+  if (row_blocks > 65535) return FSB_ERR_TOO_LARGE;
   const int vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && ldw % 8 == 0;
-  mx4_quant_weight_kernel<<<grid, 128, 0, stream>>>(static_cast<const __nv_bfloat16*>(w), static_cast<uint8_t*>(q),
-                                                    static_cast<uint8_t*>(tile_exp), static_cast<uint8_t*>(fwd),
-                                                    static_cast<uint8_t*>(dgrad), rows, cols, ldw, vec);
+  const bool wide = col_blocks * row_blocks >= 148 * 4;      // the blocks of four tiles a warp fill the SMs
+  auto kernel = wide ? mx4_quant_weight_kernel<4> : mx4_quant_weight_kernel<1>;
+  kernel<<<dim3(wide ? col_blocks : 4 * col_blocks, static_cast<unsigned>(row_blocks)), 128, 0, stream>>>(
+      static_cast<const __nv_bfloat16*>(w), static_cast<uint8_t*>(q), static_cast<uint8_t*>(tile_exp), static_cast<uint8_t*>(fwd),
+      static_cast<uint8_t*>(dgrad), rows, cols, ldw, vec);
   return ok();
 }
 
@@ -666,12 +737,17 @@ FSB_API int fsb_mx4_expand(const void* q, const void* scales, void* out, long lo
   if (K <= 0 || K % 32 != 0 || T < 0 || ldq % 4 != 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0 || kind < 0 || kind > 2)
     return FSB_ERR_BAD_ARG;
   if (T == 0) return FSB_OK;
-  const long long blocks = (T * (K / 8) + 255) / 256;
+  const long long units = T * (K / (kind == 0 ? 16 : 8)), blocks = ((units + EXPAND_UNITS - 1) / EXPAND_UNITS + 255) / 256;
   if (blocks > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
-  mx4_expand_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const uint8_t*>(q),
-                                                                      static_cast<const uint8_t*>(scales), out, T, K, ldq,
-                                                                      (K + 127) / 128, kind);
-  return ok();
+  auto run = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales),
+                                                              out, T, K, ldq, (K + 127) / 128);
+    return ok();
+  };
+  const bool small = units < (1ll << 31);
+  if (kind == 0) return small ? run(mx4_expand_kernel<0, unsigned>) : run(mx4_expand_kernel<0, long long>);
+  if (kind == 1) return small ? run(mx4_expand_kernel<1, unsigned>) : run(mx4_expand_kernel<1, long long>);
+  return small ? run(mx4_expand_kernel<2, unsigned>) : run(mx4_expand_kernel<2, long long>);
 }
 
 // d[M, N] = A B^T for codes aq [M, K / 2] and bq [N, K / 2] (row strides lda, ldb bytes, multiples of 16) with blocked scales

@@ -23,7 +23,7 @@ def rows_of(rows, cols, seed=0):
     return x.bfloat16()
 
 
-@pytest.mark.parametrize("rows,cols,pad", [(1, 32, 0), (7, 96, 0), (129, 160, 0), (300, 4128, 0), (64, 256, 8), (33, 64, 3), (257, 2048, 1)])
+@pytest.mark.parametrize("rows,cols,pad", [(1, 32, 0), (7, 96, 0), (129, 160, 0), (300, 4128, 0), (64, 256, 8), (33, 64, 3), (257, 2048, 1), (2500, 4128, 0)])
 def test_quantisers_match_the_restatement_bitwise(rows, cols, pad):
     """Odd sizes, groups and rows that end inside a scale block, row strides and bases off the 16-byte grid."""
     x = rows_of(rows, cols + 32, 3)[:, pad:pad + cols]
