@@ -316,7 +316,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     if (part == 0) {
       if (tid == 0) {
         logprob[row] = entropy[row] = 0.f;
-        stats[row] = make_float2(0.f, 0.f);
+        if (stats) stats[row] = make_float2(0.f, 0.f);
       }
       if (tid < k) {
         top_lp[row * k + tid] = 0.f;
@@ -471,7 +471,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   if (tid == 0) {
     logprob[row] = inside ? (xt - all.m) * inv_t - log_s : __uint_as_float(0x7fc00000u);
     entropy[row] = H;
-    stats[row] = make_float2(all.m, log_s);
+    if (stats) stats[row] = make_float2(all.m, log_s);
   }
   if constexpr (TOP) {
     if (tid < k) {
@@ -587,7 +587,7 @@ inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LA
 }  // namespace
 
 // kind: 0 bf16, 1 fp16, 2 fp32. x [T, V] with row stride ld elements; logprob, entropy [T]; stats [T, 2] (maximum
-// and log s, for the backward pass); top_lp, top [T, k].
+// and log s, for the backward pass; may be null); top_lp, top [T, k].
 FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target, long long T, int V, long long ld, float inv_t,
                                int k, long long ignore_index, float* logprob, float* entropy, void* stats, float* top_lp,
                                long long* top, cudaStream_t stream) {

@@ -15,6 +15,10 @@
 namespace {
 using namespace fsb;
 
+// Waits for the kernel that this one was launched behind, where it may start before that one ends; nothing otherwise.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Biased exponent from the bits of amax (not negative). 0x7f800000 and above: an infinity or a NaN.
 __device__ __forceinline__ uint32_t mx4_exponent(uint32_t bits) {
   if (bits >= 0x7f800000u) return 255u;
@@ -67,6 +71,7 @@ template <typename I>
 __global__ void __launch_bounds__(256)
 mx4_quant_act_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scales, long long T,
                      int K, long long ldx, int n_gb, int vec) {
+  let_next_kernel_start();
   const I units = n_gb * 8;                               // pieces of a padded row
   const I total = static_cast<I>((T + 127) / 128 * 128) * units, share = total / UNITS;   // both multiples of 8
   const I i0 = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -234,14 +239,20 @@ template <int BN>
 struct Tile {
   static constexpr int A_STAGE = BM * KB, B_STAGE = BN * KB;
   static constexpr int STAGE_BYTES = A_STAGE + B_STAGE + 2 * SF_BYTES;   // a multiple of 1 KB for BN >= 16 in steps of 8
-  static constexpr int STAGES = 4;
+  static constexpr int STAGES = 4;                                       // two CTAs fit an SM (BN = 128: one)
+  // steps of a CTA along K that are worth the joining of the parts (measured with 2, 4, 8 and without a split: 32 x 6144 x 4096
+  // 12.9, 9.4, 9.7, 10.4 us; 64 x 4096 x 14336 13.7, 13.7, 13.1, 22.9; 128 x 6144 x 4096 20.9, 20.9, 14.1, 12.6)
+  static constexpr int LEAST = BN == 128 ? 14 : BN == 64 ? 8 : 4;
   static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
   static constexpr int SF_COL0 = BN < 32 ? 32 : BN;                      // first scale column
   static constexpr int TMEM_COLS = BN <= 64 ? 128 : 256;                 // accumulator + two sets of 8 + 8 scale columns
 };
 
+constexpr int MAX_SPLIT = 8;                        // CTAs along K (a portable cluster)
+
 struct Args {
   int M, N, K;
+  int split, chunk;                                 // CTAs of a cluster along K, 256-deep steps of each
   void* d;
   long long ldd;
   int d_fp32;
@@ -273,8 +284,67 @@ __device__ __forceinline__ constexpr uint32_t make_idesc_mx4(uint32_t m, uint32_
   return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (sf_id << 29);
 }
 
+// Four neighbouring columns of row t.
+__device__ __forceinline__ void store4(const Args& args, int t, int n, const float4& v) {
+  const long long at = static_cast<long long>(t) * args.ldd + n;
+  if (args.d_fp32) {
+    float* d = static_cast<float*>(args.d) + at;
+    if (n + 4 <= args.N && (reinterpret_cast<uintptr_t>(d) & 15) == 0) {
+      *reinterpret_cast<float4*>(d) = v;
+      return;
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < args.N) d[i] = f[i];
+  } else {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(args.d) + at;
+    if (n + 4 <= args.N && (reinterpret_cast<uintptr_t>(d) & 7) == 0) {
+      *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      return;
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < args.N) d[i] = __float2bfloat16(f[i]);
+  }
+}
+// Epilogue of the one-SM kernels: the 128 threads of the epilogue warps have left their CTA's sums [rows][128] at `smem` (a
+// thread there has one weight row, 2 bytes of each output row; here it stores 8 of one). With several CTAs along K the cluster's
+// sums are added in CTA order and the CTAs divide the rows; all parts' 16 bytes are on their way before the first is added.
+__device__ __forceinline__ void store_rows(const Args& args, const uint8_t* smem, int part, int t0, int rows, int n0, int thread) {
+  const int n = thread % 32 * 4;
+  if (args.split == 1) {
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 4
+    for (int t = thread / 32; t < rows; t += 4) store4(args, t0 + t, n0 + n, *reinterpret_cast<const float4*>(smem + (t * BM + n) * 4));
+    return;
+  }
+  const int per = (rows + args.split - 1) / args.split, end = min((part + 1) * per, rows);
+#pragma unroll 2
+  for (int t = part * per + thread / 32; t < end; t += 4) {
+    const uint32_t own = smem_u32(smem) + (t * BM + n) * 4;
+    float4 o[MAX_SPLIT], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < MAX_SPLIT; ++p) {
+      o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p < args.split)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(o[p].x), "=f"(o[p].y), "=f"(o[p].z), "=f"(o[p].w) : "r"(map_to_cta(own, p)));
+    }
+#pragma unroll
+    for (int p = 0; p < MAX_SPLIT; ++p) {
+      sum.x += o[p].x;
+      sum.y += o[p].y;
+      sum.z += o[p].z;
+      sum.w += o[p].w;
+    }
+    store4(args, t0 + t, n0 + n, sum);
+  }
+}
+
 template <int BN>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(NUM_THREADS)
 gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_sfw, const __grid_constant__ CUtensorMap map_sfx, const Args args) {
   using S = Tile<BN>;
@@ -288,8 +358,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tw = blockIdx.x, tx = blockIdx.y;
+  const int tw = blockIdx.x / args.split, part = blockIdx.x % args.split, tx = blockIdx.y, rows = min(BN, args.M - tx * BN);
   const int num_kb = (args.K + BK - 1) / BK;
+  const int kb0 = min(part * args.chunk, num_kb), steps = min(kb0 + args.chunk, num_kb) - kb0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
@@ -313,29 +384,37 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     if (lane == 0) {
       tma_prefetch_desc(&map_w);
       tma_prefetch_desc(&map_x);
-      for (int kb = 0; kb < num_kb; ++kb) {
-        const int s = kb % S::STAGES;
-        if (!mbar_wait(&empty_bar[s], ((kb / S::STAGES) & 1) ^ 1, abort_flag)) {
-          atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_EMPTY);
-          *abort_flag = 1;
-          break;
-        }
+      auto load_weight = [&](int i) {
+        const int s = i % S::STAGES, kb = kb0 + i;
         uint8_t* sa = smem + s * S::STAGE_BYTES;
-        uint8_t* sb = sa + S::A_STAGE;
-        uint8_t* ssf = sb + S::B_STAGE;
         mbar_expect_tx(&full_bar[s], S::STAGE_BYTES);
         tma_load_2d(sa, &map_w, &full_bar[s], kb * KB, tw * BM);
+        tma_load_2d(sa + S::A_STAGE + S::B_STAGE, &map_sfw, &full_bar[s], kb * 256, tw);   // 256 words: two blocks
+      };
+      const int ahead = min(steps, S::STAGES);
+      for (int i = 0; i < ahead; ++i) load_weight(i);          // does not wait for the rows' quantiser
+      wait_for_previous_kernel();
+      for (int i = 0; i < steps; ++i) {
+        const int s = i % S::STAGES, kb = kb0 + i;
+        if (i >= ahead) {
+          if (!mbar_wait(&empty_bar[s], ((i / S::STAGES) & 1) ^ 1, abort_flag)) {
+            atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_EMPTY);
+            *abort_flag = 1;
+            break;
+          }
+          load_weight(i);
+        }
+        uint8_t* sb = smem + s * S::STAGE_BYTES + S::A_STAGE;
         tma_load_2d(sb, &map_x, &full_bar[s], kb * KB, tx * BN);
-        tma_load_2d(ssf, &map_sfw, &full_bar[s], kb * 256, tw);                        // 256 words: two blocks
-        tma_load_2d(ssf + SF_BYTES, &map_sfx, &full_bar[s], kb * 256, tx * BN / 128);
+        tma_load_2d(sb + S::B_STAGE + SF_BYTES, &map_sfx, &full_bar[s], kb * 256, tx * BN / 128);
       }
     }
   } else if (warp == 1) {
     // The whole warp walks the loop; one elected lane issues the tcgen05 instructions.
-    bool ok = true;
-    for (int kb = 0; kb < num_kb; ++kb) {
-      const int s = kb % S::STAGES;
-      if (!mbar_wait(&full_bar[s], (kb / S::STAGES) & 1, abort_flag)) {
+    bool ok = steps > 0;
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % S::STAGES;
+      if (!mbar_wait(&full_bar[s], (i / S::STAGES) & 1, abort_flag)) {
         if (lane == 0) {
           atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_FULL);
           *abort_flag = 1;
@@ -348,7 +427,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       const uint64_t da = make_smem_desc_sw128(sa, 16, 1024);
       const uint64_t db = make_smem_desc_sw128(sa + S::A_STAGE, 16, 1024);
       const uint32_t ssf = sa + S::A_STAGE + S::B_STAGE;
-      const uint32_t tsf = tmem_base + S::SF_COL0 + (kb & 1) * 16;   // 2 x 4 columns of weight scales, 2 x 4 of row scales
+      const uint32_t tsf = tmem_base + S::SF_COL0 + (i & 1) * 16;   // 2 x 4 columns of weight scales, 2 x 4 of row scales
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -358,7 +437,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           umma_mxf4(tmem_base, da + 2 * k, db + 2 * k, make_idesc_mx4(BM, BN, (k & 1) * 2), tsf + 4 * (k >> 1),
-                    tsf + 8 + 4 * (k >> 1), (kb | k) != 0);
+                    tsf + 8 + 4 * (k >> 1), (i | k) != 0);
         umma_commit(&empty_bar[s]);
       }
       __syncwarp();
@@ -370,29 +449,37 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   } else {
     const int quarter = warp & 3;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const int n = tw * BM + quarter * 32 + lane;
-    if (!mbar_wait_warp(tmem_full, 0, abort_flag)) {
-      if (lane == 0) {
-        atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_TMEM_FULL);
-        *abort_flag = 1;
-      }
-    } else {
-      tc_fence_after();
+    const bool done = steps > 0 && mbar_wait_warp(tmem_full, 0, abort_flag);
+    if (steps > 0 && !done && lane == 0) {
+      atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_TMEM_FULL);
+      *abort_flag = 1;
+    }
+    tc_fence_after();
+    uint32_t* sums = reinterpret_cast<uint32_t*>(smem) + quarter * 32 + lane;   // the stages are free by now
 #pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 16) {
-        uint32_t v[16];
+    for (int c0 = 0; c0 < BN; c0 += 16) {
+      if (c0 >= rows) break;
+      uint32_t v[16];
+      if (done) {
         tmem_ld_32x16(t_row + c0, v);
         tmem_ld_wait();
-        if (n >= args.N) continue;
+      } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const long long t = static_cast<long long>(tx) * BN + c0 + i;
-          if (t >= args.M) break;
-          if (args.d_fp32) static_cast<float*>(args.d)[t * args.ldd + n] = __uint_as_float(v[i]);
-          else static_cast<__nv_bfloat16*>(args.d)[t * args.ldd + n] = __float2bfloat16(__uint_as_float(v[i]));
-        }
+        for (int i = 0; i < 16; ++i) v[i] = 0;                 // nothing along K for this CTA
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sums[(c0 + i) * BM] = v[i];
     }
+    tc_fence_before();
+  }
+  if (args.split > 1) {
+    __syncwarp();
+    cluster_sync_all();
+  }
+  if (warp >= 2) store_rows(args, smem, part, tx * BN, rows, tw * BM, static_cast<int>(threadIdx.x) - 64);
+  if (args.split > 1) {
+    __syncwarp();
+    cluster_sync_all();                                        // the others' sums have been read
   }
   tc_fence_before();
   __syncthreads();
@@ -404,6 +491,182 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
     tc_fence_after();
     tmem_dealloc(tmem_base, S::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ few rows: quantised on the way, split along K
+// Up to 16 rows of bf16 against a weight in one launch. The CTAs of a cluster share a tile of 128 weight rows and divide its
+// K; each quantises its own columns of the rows straight into shared memory (the 128-byte swizzle's order: one group is one
+// 16-byte chunk) while the weight streams in, and the partial sums meet in the cluster's shared memory, added in CTA order.
+// Bound by the weight's bytes where there are enough of them, else by the latency of one load, one chain of MMAs and the exchange.
+constexpr int F_BN = 16, F_STAGES = 3;
+constexpr int F_STAGE_BYTES = BM * KB + SF_BYTES;            // weight codes and scales: 17 KB
+constexpr int F_ROW_BYTES = F_BN * KB + SF_BYTES;            // the rows' codes and scales of 256 columns: 3 KB
+constexpr int F_SF_COL0 = 32, F_TMEM_COLS = 64;
+constexpr int FEW_GROUPS = 512;                                // most groups a CTA quantises, four a thread
+constexpr int few_smem(int chunk) { return F_STAGES * F_STAGE_BYTES + chunk * F_ROW_BYTES + 1024 + 256; }
+
+__global__ void __launch_bounds__(NUM_THREADS)
+linear_mxfp4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sfw,
+                        const __nv_bfloat16* __restrict__ x, long long ldx, int vec, const Args args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* rows_q = smem + F_STAGES * F_STAGE_BYTES;          // [chunk][16 rows][128 bytes]
+  uint8_t* rows_sf = rows_q + args.chunk * F_BN * KB;              // [chunk][two scale blocks]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(rows_sf + args.chunk * SF_BYTES);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + F_STAGES;
+  uint64_t* rows_ready = bars + 2 * F_STAGES;
+  uint64_t* tmem_full = bars + 2 * F_STAGES + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * F_STAGES + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tw = blockIdx.x / args.split, part = blockIdx.x % args.split;
+  const int num_kb = (args.K + BK - 1) / BK;
+  const int kb0 = min(part * args.chunk, num_kb), steps = min(kb0 + args.chunk, num_kb) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < F_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(rows_ready, 128);
+    mbar_init(tmem_full, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, F_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  float acc[F_BN];                                            // the epilogue warps' sums: one weight row, 16 rows of x
+#pragma unroll
+  for (int i = 0; i < F_BN; ++i) acc[i] = 0.f;
+  const int quarter = warp & 3, n_local = quarter * 32 + lane;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&map_w);
+      for (int i = 0; i < steps; ++i) {
+        const int s = i % F_STAGES;
+        if (!mbar_wait(&empty_bar[s], ((i / F_STAGES) & 1) ^ 1, abort_flag)) {
+          atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_EMPTY);
+          *abort_flag = 1;
+          break;
+        }
+        uint8_t* sa = smem + s * F_STAGE_BYTES;
+        mbar_expect_tx(&full_bar[s], F_STAGE_BYTES);
+        tma_load_2d(sa, &map_w, &full_bar[s], (kb0 + i) * KB, tw * BM);
+        tma_load_2d(sa + BM * KB, &map_sfw, &full_bar[s], (kb0 + i) * 256, tw);
+      }
+    }
+  } else if (warp == 1) {
+    bool ok = steps > 0;
+    if (ok && !mbar_wait(rows_ready, 0, abort_flag)) {
+      if (lane == 0) {
+        atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_FULL);
+        *abort_flag = 1;
+      }
+      ok = false;
+    }
+    for (int i = 0; i < steps && ok; ++i) {
+      const int s = i % F_STAGES;
+      if (!mbar_wait(&full_bar[s], (i / F_STAGES) & 1, abort_flag)) {
+        if (lane == 0) {
+          atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_FULL);
+          *abort_flag = 1;
+        }
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sa = smem_u32(smem + s * F_STAGE_BYTES);
+      const uint64_t da = make_smem_desc_sw128(sa, 16, 1024);
+      const uint64_t db = make_smem_desc_sw128(smem_u32(rows_q + i * F_BN * KB), 16, 1024);
+      const uint32_t sfw = sa + BM * KB, sfx = smem_u32(rows_sf + i * SF_BYTES);
+      const uint32_t tsf = tmem_base + F_SF_COL0 + (i & 1) * 16;
+      if (elect_one()) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tmem_cp_32x128b_x4(tsf + 4 * h, make_sf_desc(sfw + 512 * h));
+          tmem_cp_32x128b_x4(tsf + 8 + 4 * h, make_sf_desc(sfx + 512 * h));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_mxf4(tmem_base, da + 2 * k, db + 2 * k, make_idesc_mx4(BM, F_BN, (k & 1) * 2), tsf + 4 * (k >> 1),
+                    tsf + 8 + 4 * (k >> 1), (i | k) != 0);
+        umma_commit(&empty_bar[s]);
+      }
+      __syncwarp();
+    }
+    if (ok) {
+      if (elect_one()) umma_commit(tmem_full);
+      __syncwarp();
+    }
+  } else if (steps > 0) {
+    // a thread per group of 32 columns of a row; groups past K hold zeros with scale 1 (rows past M are never read)
+    const int groups = steps * 8;
+    for (int i = threadIdx.x - 64; i < args.M * groups; i += 128) {
+      const int r = i / groups, g = i - r * groups, kb = g >> 3, in = g & 7;
+      const int col = (kb0 + kb) * BK + in * 32;
+      uint4 v[4];
+      uint32_t m = 0;
+      const bool live = col < args.K;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = live ? load8_any(x + r * ldx + col + 8 * j, vec) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = amax8_bits(v[j], m);
+      const uint32_t e = mx4_exponent(m);
+      const float inv = mx4_inv(e);
+      *reinterpret_cast<uint4*>(rows_q + kb * F_BN * KB + r * KB + ((in ^ (r & 7)) << 4)) =
+          make_uint4(quant8_fp4(v[0], inv), quant8_fp4(v[1], inv), quant8_fp4(v[2], inv), quant8_fp4(v[3], inv));
+      rows_sf[kb * SF_BYTES + (in >> 2) * 512 + r * 16 + (in & 3)] = live ? static_cast<uint8_t>(e) : 127;
+    }
+    fence_proxy_async_smem();                                 // written by threads, read by the tensor core
+    mbar_arrive(rows_ready);
+    if (!mbar_wait_warp(tmem_full, 0, abort_flag)) {
+      if (lane == 0) {
+        atomicExch(args.status, FSB_ERR_WAIT_TIMEOUT_TMEM_FULL);
+        *abort_flag = 1;
+      }
+    } else {
+      tc_fence_after();
+      uint32_t v[16];
+      tmem_ld_32x16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16), v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < F_BN; ++i) acc[i] = __uint_as_float(v[i]);
+    }
+    tc_fence_before();
+  }
+  if (warp >= 2) {
+#pragma unroll
+    for (int i = 0; i < F_BN; ++i) reinterpret_cast<float*>(smem)[i * BM + n_local] = acc[i];   // the first stage is free by now
+  }
+  if (args.split > 1) {
+    __syncwarp();
+    cluster_sync_all();
+  }
+  if (warp >= 2) store_rows(args, smem, part, 0, args.M, tw * BM, static_cast<int>(threadIdx.x) - 64);
+  if (args.split > 1) {
+    __syncwarp();
+    cluster_sync_all();                                       // the others' sums have been read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (*abort_flag) {
+      const unsigned long long t0 = clock64();
+      while (clock64() - t0 < 2000000ull) {
+      }
+    }
+    tc_fence_after();
+    tmem_dealloc(tmem_base, F_TMEM_COLS);
   }
 }
 
@@ -476,6 +739,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       tma_prefetch_desc(&map_b);
       tma_prefetch_desc(&map_sfa);
       tma_prefetch_desc(&map_sfb);
+      wait_for_previous_kernel();
       uint32_t it = 0;
       bool ok = true;
       for (int tile = tile0; tile < num_tiles && ok; tile += tile_step) {
@@ -648,28 +912,85 @@ int scales_map(CUtensorMap* map, const void* sf, long long rows, int K, int box_
   return fsb_make_tmap_2d_plain(map, sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (rows + 127) / 128, words, words, box_rows, 256);
 }
 
-template <int BN>
-int launch(const void* aq, const void* sfa, const void* bq, const void* sfb, const Args& a, long long lda, long long ldb,
-           cudaStream_t stream) {
-  static bool raised[64] = {false};
+// CTAs along K for `tiles` tiles: as many as there are places for, each with `least` 256-deep steps or more.
+int k_split(long long tiles, int num_kb, int least, int places) {
+  const int most = min(MAX_SPLIT, max(1, num_kb / least)), split = static_cast<int>(max(1ll, min(static_cast<long long>(most), places / tiles)));
+  const int chunk = (num_kb + split - 1) / split;
+  return (num_kb + chunk - 1) / chunk;
+}
+
+// Launch of a kernel whose clusters are `split` CTAs along x. PDL: it may start while the kernel before it in the stream still
+// runs, and waits for that kernel's results itself.
+template <typename... P, typename... A>
+int launch_split(void (*kernel)(P...), dim3 grid, int smem, int split, bool pdl, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2] = {};
+  cfg.attrs = at;
+  if (split > 1) {
+    cudaLaunchAttribute& c = at[cfg.numAttrs++];
+    c.id = cudaLaunchAttributeClusterDimension;
+    c.val.clusterDim.x = split;
+    c.val.clusterDim.y = 1;
+    c.val.clusterDim.z = 1;
+  }
+  if (pdl) {
+    cudaLaunchAttribute& c = at[cfg.numAttrs++];
+    c.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    c.val.programmaticStreamSerializationAllowed = 1;
+  }
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args...);
+  const int rc = ok();   // also clears the error of a launch that failed
+  return err == cudaSuccess ? rc : static_cast<int>(FSB_ERR_LAUNCH);
+}
+// The kernel's shared-memory limit raised once per device.
+template <typename Kernel>
+bool raise_smem(Kernel kernel, bool (&raised)[64], int bytes) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return FSB_ERR_BAD_ARG;
-  if (!raised[dev]) {
-    if (cudaFuncSetAttribute(gemm_mxfp4_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<BN>::SMEM) != cudaSuccess)
-      return FSB_ERR_LAUNCH;
-    raised[dev] = true;
-  }
+  if (dev < 0 || dev >= 64) return false;
+  if (!raised[dev]) raised[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  return raised[dev];
+}
+
+// FSB_ERR_TOO_LARGE: the rows' share of a CTA is more than its threads quantise while the weight arrives, or than fits.
+int launch_few(const void* x, const void* bq, const void* sfb, Args a, long long ldx, long long ldb, cudaStream_t stream) {
+  static bool raised[64] = {false};
+  constexpr int MOST_SMEM = 227 * 1024;
+  if (!raise_smem(linear_mxfp4_few_kernel, raised, MOST_SMEM)) return FSB_ERR_LAUNCH;
+  const int tiles = (a.N + BM - 1) / BM, num_kb = (a.K + BK - 1) / BK;
+  a.split = k_split(tiles, num_kb, 2, 296);
+  a.chunk = (num_kb + a.split - 1) / a.split;
+  if (few_smem(a.chunk) > MOST_SMEM || a.M * a.chunk * 8 > FEW_GROUPS) return FSB_ERR_TOO_LARGE;
+  CUtensorMap map_w, map_sfw;
+  int rc = codes_map(&map_w, bq, a.N, a.K, ldb, BM);
+  if (rc == FSB_OK) rc = scales_map(&map_sfw, sfb, a.N, a.K, 1);
+  if (rc != FSB_OK) return rc;
+  const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx % 8 == 0;
+  return launch_split(linear_mxfp4_few_kernel, dim3(tiles * a.split), few_smem(a.chunk), a.split, false, stream, map_w, map_sfw,
+                      static_cast<const __nv_bfloat16*>(x), ldx, vec, a);
+}
+
+template <int BN>
+int launch(const void* aq, const void* sfa, const void* bq, const void* sfb, Args a, long long lda, long long ldb, bool pdl,
+           cudaStream_t stream) {
+  static bool raised[64] = {false};
+  if (!raise_smem(gemm_mxfp4_kernel<BN>, raised, Tile<BN>::SMEM)) return FSB_ERR_LAUNCH;
   CUtensorMap map_w, map_x, map_sfw, map_sfx;
   int rc = codes_map(&map_w, bq, a.N, a.K, ldb, BM);
   if (rc == FSB_OK) rc = codes_map(&map_x, aq, a.M, a.K, lda, BN);
   if (rc == FSB_OK) rc = scales_map(&map_sfw, sfb, a.N, a.K, 1);
   if (rc == FSB_OK) rc = scales_map(&map_sfx, sfa, a.M, a.K, 1);
   if (rc != FSB_OK) return rc;
-  const dim3 grid((a.N + BM - 1) / BM, (a.M + BN - 1) / BN);
-  if (grid.y > 65535) return FSB_ERR_TOO_LARGE;
-  gemm_mxfp4_kernel<BN><<<grid, NUM_THREADS, Tile<BN>::SMEM, stream>>>(map_w, map_x, map_sfw, map_sfx, a);
-  return ok();
+  const int tiles_w = (a.N + BM - 1) / BM, tiles_x = (a.M + BN - 1) / BN, num_kb = (a.K + BK - 1) / BK;
+  if (tiles_x > 65535) return FSB_ERR_TOO_LARGE;
+  a.split = k_split(static_cast<long long>(tiles_w) * tiles_x, num_kb, Tile<BN>::LEAST, BN == 128 ? 148 : 296);
+  a.chunk = (num_kb + a.split - 1) / a.split;
+  return launch_split(gemm_mxfp4_kernel<BN>, dim3(tiles_w * a.split, tiles_x), Tile<BN>::SMEM, a.split, pdl, stream, map_w, map_x,
+                      map_sfw, map_sfx, a);
 }
 
 // Clusters of the pair kernel that fit the current device at once (-1: unusable).
@@ -682,7 +1003,7 @@ int resident_pairs() {
   return pairs[dev];
 }
 int launch_pairs(const void* aq, const void* sfa, const void* bq, const void* sfb, const Args& a, long long lda, long long ldb,
-                 int pairs, cudaStream_t stream) {
+                 int pairs, bool pdl, cudaStream_t stream) {
   CUtensorMap map_a, map_b, map_sfa, map_sfb;
   int rc = codes_map(&map_a, aq, a.M, a.K, lda, BM);
   if (rc == FSB_OK) rc = codes_map(&map_b, bq, a.N, a.K, ldb, BM);
@@ -690,8 +1011,35 @@ int launch_pairs(const void* aq, const void* sfa, const void* bq, const void* sf
   if (rc == FSB_OK) rc = scales_map(&map_sfb, sfb, a.N, a.K, 2);
   if (rc != FSB_OK) return rc;
   const int tiles = ((a.M + 2 * BM - 1) / (2 * BM)) * ((a.N + P_BN - 1) / P_BN);
-  gemm_mxfp4_pair_kernel<<<2 * (tiles < pairs ? tiles : pairs), P_THREADS, P_SMEM, stream>>>(map_a, map_b, map_sfa, map_sfb, a);
-  return ok();
+  cudaLaunchConfig_t cfg{};                                  // the cluster's size is the kernel's own
+  cfg.gridDim = dim3(2 * (tiles < pairs ? tiles : pairs));
+  cfg.blockDim = dim3(P_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = P_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_mxfp4_pair_kernel, map_a, map_b, map_sfa, map_sfb, a);
+  rc = ok();
+  return err == cudaSuccess ? rc : static_cast<int>(FSB_ERR_LAUNCH);
+}
+// pdl: the kernel before this one in the stream is the quantiser of a.
+int product(const void* aq, const void* sfa, const void* bq, const void* sfb, const Args& a, long long lda, long long ldb, bool pdl,
+            cudaStream_t stream) {
+  if (a.M <= 16) return launch<16>(aq, sfa, bq, sfb, a, lda, ldb, pdl, stream);
+  if (a.M <= 32) return launch<32>(aq, sfa, bq, sfb, a, lda, ldb, pdl, stream);
+  if (a.M <= 64) return launch<64>(aq, sfa, bq, sfb, a, lda, ldb, pdl, stream);
+  // More 128 x 128 tiles than SMs: pairs of them, on SM pairs. One SM a tile against pairs, with the quantiser: 256 x 6144 x 4096
+  // (96 tiles) 12.8 / 15.3 us, 512 x 4096 x 4096 (128) 12.8 / 14.2, 512 x 6144 x 4096 (192) 22.2 / 15.9, 128 x 28672 x 4096 (224)
+  // 25.2 / 23.0, 777 x 5000 x 2080 (280) 20.6 / 18.0, 1024 x 4096 x 4096 (256) 23.1 / 15.4.
+  const long long tiles = static_cast<long long>((a.M + BM - 1) / BM) * ((a.N + BM - 1) / BM);
+  if (tiles > 148) {
+    const int pairs = resident_pairs();
+    if (pairs > 0) return launch_pairs(aq, sfa, bq, sfb, a, lda, ldb, pairs, pdl, stream);
+  }
+  return launch<128>(aq, sfa, bq, sfb, a, lda, ldb, pdl, stream);
 }
 }  // namespace
 
@@ -758,15 +1106,24 @@ FSB_API int fsb_gemm_mxfp4(const void* aq, const void* sfa, const void* bq, cons
   if ((reinterpret_cast<uintptr_t>(sfa) | reinterpret_cast<uintptr_t>(sfb) | reinterpret_cast<uintptr_t>(aq) |
        reinterpret_cast<uintptr_t>(bq)) & 15)
     return FSB_ERR_BAD_ARG;
-  Args a;
-  a.M = M; a.N = N; a.K = K;
-  a.d = d; a.ldd = ldd; a.d_fp32 = d_fp32; a.status = status;
-  if (M <= 16) return launch<16>(aq, sfa, bq, sfb, a, lda, ldb, stream);
-  if (M <= 32) return launch<32>(aq, sfa, bq, sfb, a, lda, ldb, stream);
-  if (M <= 64) return launch<64>(aq, sfa, bq, sfb, a, lda, ldb, stream);
-  if (M > 512) {
-    const int pairs = resident_pairs();
-    if (pairs > 0) return launch_pairs(aq, sfa, bq, sfb, a, lda, ldb, pairs, stream);
+  const Args a{M, N, K, 1, 0, d, ldd, d_fp32, status};
+  return product(aq, sfa, bq, sfb, a, lda, ldb, false, stream);
+}
+
+// d[M, N] = Q(x) B^T for bf16 x [M, K] with row stride ldx: the quantiser and the product, in one launch for up to 16 rows.
+// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes on a 16-byte boundary.
+FSB_API int fsb_mxfp4_linear(const void* x, long long ldx, const void* bq, long long ldb, const void* sfb, void* d, long long ldd,
+                             void* scratch, int M, int N, int K, int* status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || ldb % 16 != 0) return FSB_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(sfb) | reinterpret_cast<uintptr_t>(bq)) & 15) return FSB_ERR_BAD_ARG;
+  const Args a{M, N, K, 1, 0, d, ldd, 0, status};
+  if (M <= F_BN) {
+    const int rc = launch_few(x, bq, sfb, a, ldx, ldb, stream);
+    if (rc != FSB_ERR_TOO_LARGE) return rc;
   }
-  return launch<128>(aq, sfa, bq, sfb, a, lda, ldb, stream);
+  if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15)) return FSB_ERR_BAD_ARG;
+  uint8_t* q = static_cast<uint8_t*>(scratch);
+  uint8_t* sf = q + static_cast<long long>(M) * (K / 2);      // K / 2 is a multiple of 16
+  const int rc = fsb_mx4_quant_act(x, q, sf, M, K, ldx, stream);
+  return rc == FSB_OK ? product(q, sf, bq, sfb, a, K / 2, ldb, true, stream) : rc;
 }

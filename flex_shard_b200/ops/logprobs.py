@@ -2,8 +2,8 @@
 (``csrc/logprobs.cu``). The counterpart of ``cross_entropy`` where a value per token is wanted: policy gradients,
 distillation on a teacher's alternatives, scoring.
 
-CPU tensors, and tensors that a kernel cannot be given (batched gradients, ``torch.func`` transforms), take a PyTorch
-restatement.
+CPU tensors, and tensors that a kernel cannot be given (batched gradients, ``torch.func`` transforms, forward-mode
+derivatives), take a PyTorch restatement.
 """
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import count_launch
@@ -84,21 +85,30 @@ def _restated_gradient(x, target, top, stats, entropy, temperature, ignore_index
     return (torch.where(live[:, None], dz, 0.0) / temperature).to(x.dtype)
 
 
+def _forward(x, target, temperature, k, ignore_index, stats):
+    """``stats`` [T, 2] takes the numbers of a row that the gradient starts from (``None``: not wanted)."""
+    _ensure()
+    T, V = x.shape
+    dev = x.device
+    logprob = torch.empty(T, dtype=torch.float32, device=dev)
+    entropy = torch.empty(T, dtype=torch.float32, device=dev)
+    top_lp = torch.empty(T, k, dtype=torch.float32, device=dev)
+    top = torch.empty(T, k, dtype=torch.int64, device=dev)
+    with _lib.device_of(x):
+        rc = _lib.load().fsb_token_logprobs(x.data_ptr(), _KINDS[x.dtype], target.data_ptr(), T, V, x.stride(0), 1.0 / temperature,
+                                            k, ignore_index, logprob.data_ptr(), entropy.data_ptr(),
+                                            None if stats is None else stats.data_ptr(), top_lp.data_ptr(), top.data_ptr(),
+                                            _lib.stream_ptr(dev))
+    _lib.check(rc, "fsb_token_logprobs")
+    count_launch(int(T > 0))
+    return logprob, entropy, top_lp, top
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, target, temperature, k, ignore_index):
-        _ensure()
-        T, V = x.shape
-        dev = x.device
-        f32 = lambda *n: torch.empty(*n, dtype=torch.float32, device=dev)  # noqa: E731
-        logprob, entropy, stats, top_lp = f32(T), f32(T), f32(T, 2), f32(T, k)
-        top = torch.empty(T, k, dtype=torch.int64, device=dev)
-        with _lib.device_of(x):
-            rc = _lib.load().fsb_token_logprobs(x.data_ptr(), _KINDS[x.dtype], target.data_ptr(), T, V, x.stride(0),
-                                                1.0 / temperature, k, ignore_index, logprob.data_ptr(), entropy.data_ptr(),
-                                                stats.data_ptr(), top_lp.data_ptr(), top.data_ptr(), _lib.stream_ptr(dev))
-        _lib.check(rc, "fsb_token_logprobs")
-        count_launch(int(T > 0))
+        stats = torch.empty(x.shape[0], 2, dtype=torch.float32, device=x.device)
+        logprob, entropy, top_lp, top = _forward(x, target, temperature, k, ignore_index, stats)
         ctx.save_for_backward(x, target, top, stats, entropy)
         ctx.cfg = (temperature, ignore_index)
         ctx.mark_non_differentiable(top)
@@ -166,12 +176,23 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, *, temperature: f
     temperature = float(temperature)
     if not 1e-30 <= temperature <= 1e30:        # its reciprocal is an fp32 number
         raise ValueError(f"temperature must be positive and finite (1e-30 to 1e30), got {temperature}")
-    x, t = logits.reshape(-1, V), target.reshape(-1).long()
-    if x.is_cuda and _lib.plain(logits, target):
-        if x.stride(1) != 1:
+    lead = target.shape
+    x, t = logits, target
+    if len(lead) != 1:
+        x, t = x.reshape(-1, V), t.reshape(-1)
+    if t.dtype != torch.int64:
+        t = t.long()
+    if x.is_cuda and _lib.plain(logits, target) and forward_ad._current_level < 0:
+        if V > 1 and x.stride(1) != 1:
             x = x.contiguous()
-        out = _TokenLogprobs.apply(x, t.contiguous(), temperature, top_k, ignore_index)
+        if not t.is_contiguous():
+            t = t.contiguous()
+        if logits.requires_grad and torch.is_grad_enabled():
+            out = _TokenLogprobs.apply(x, t, temperature, top_k, ignore_index)
+        else:
+            out = _forward(x, t, temperature, top_k, ignore_index, None)
     else:
         out = _restatement(x, t, temperature, top_k, ignore_index)
-    lead = target.shape
-    return TokenLogprobs(out[0].view(lead), out[1].view(lead), out[2].view(*lead, top_k), out[3].view(*lead, top_k))
+    if len(lead) != 1:
+        out = (out[0].view(lead), out[1].view(lead), out[2].view(*lead, top_k), out[3].view(*lead, top_k))
+    return TokenLogprobs(*out)

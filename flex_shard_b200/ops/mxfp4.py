@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import count_launch
@@ -36,6 +37,7 @@ def _ensure():
         _lib.declare("fsb_mx4_quant_act", [vp, vp, vp, i64, i32, i64, vp])
         _lib.declare("fsb_mx4_quant_weight", [vp, vp, vp, vp, vp, i32, i32, i64, vp])
         _lib.declare("fsb_mx4_expand", [vp, vp, vp, i64, i32, i64, i32, vp])
+        _lib.declare("fsb_mxfp4_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i32, vp, vp])
         _lib.declare("fsb_gemm_mxfp4", [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, vp, vp])
         _declared = True
 
@@ -55,7 +57,7 @@ def _check_operand(q: torch.Tensor, scales: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what}: codes must be a uint8 matrix [rows, cols / 2] with cols a multiple of {GROUP}, got "
                          f"{q.dtype}{tuple(q.shape)}")
     need = blocked_scale_numel(q.shape[0], 2 * q.shape[1])
-    if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.numel() < need or scales.device != q.device:
+    if scales.dtype != torch.uint8 or scales.numel() < need or not scales.is_contiguous() or scales.device != q.device:
         raise ValueError(f"{what}: scales must be at least {need} contiguous uint8 bytes in block layout on the codes' device")
 
 
@@ -234,6 +236,32 @@ def _whole_octets(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[0] % 8 == 0 else torch.nn.functional.pad(t, (0, 0, 0, -t.shape[0] % 8))
 
 
+def _product_with(x2, wq, fwd_scale):
+    """``[T, K]`` rows times the quantised weight: the forward pass of ``mxfp4_linear``."""
+    T, K = x2.shape
+    N = wq.shape[0]
+    if not x2.is_cuda:
+        return gemm_mxfp4(*mx4_quantize_act(x2), wq, fwd_scale)
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=x2.device)
+    if T == 0 or N == 0:
+        return out
+    _ensure()
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    if wq.stride(1) != 1 or wq.stride(0) % 16 or wq.data_ptr() % 16:
+        wq = wq.contiguous()
+    if fwd_scale.data_ptr() % 16:
+        fwd_scale = fwd_scale.clone()
+    scratch = torch.empty(T * (K // 2) + blocked_scale_numel(T, K), dtype=torch.uint8, device=x2.device)   # codes, scales
+    with _lib.device_of(x2):
+        rc = _lib.load().fsb_mxfp4_linear(x2.data_ptr(), x2.stride(0), wq.data_ptr(), wq.stride(0), fwd_scale.data_ptr(),
+                                          out.data_ptr(), N, scratch.data_ptr(), T, N, K,
+                                          _lib.status_word(x2.device).data_ptr(), _lib.stream_ptr(x2.device))
+    _lib.check(rc, "fsb_mxfp4_linear")
+    count_launch(2)
+    return out
+
+
 class _Mxfp4Linear(torch.autograd.Function):
     """y = x W^T in 4 bits; gradients in 8 bits with the 4-bit weights' own values (quantisation counts as the identity)."""
 
@@ -243,8 +271,7 @@ class _Mxfp4Linear(torch.autograd.Function):
         ctx.save_for_backward(x2, wq, dgrad_scale)
         ctx.xshape = x.shape
         ctx.weight = weight
-        xq, sx = mx4_quantize_act(x2)
-        return gemm_mxfp4(xq, sx, wq, fwd_scale).view(*x.shape[:-1], wq.shape[0])
+        return _product_with(x2, wq, fwd_scale).view(*x.shape[:-1], wq.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
@@ -288,15 +315,22 @@ def mxfp4_linear(x, weight, wq, fwd_scale, dgrad_scale):
     weight. Gradients run on the 8-bit products and need N and K in multiples of 128 (``x``'s) and of 8 (the weight's)."""
     if x.dtype != torch.bfloat16:
         raise ValueError(f"mxfp4_linear takes bf16 inputs, got {x.dtype}")
-    if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != 2 * wq.shape[1]:
-        raise ValueError(f"mxfp4_linear: input {tuple(x.shape)} does not match codes {tuple(wq.shape)} ([N, K / 2])")
-    N, K = wq.shape[0], x.shape[-1]
-    if torch.is_grad_enabled():
-        if x.requires_grad:
+    _check_operand(wq, fwd_scale, "mxfp4_linear")
+    N, K = wq.shape[0], 2 * wq.shape[1]
+    if x.dim() < 1 or x.shape[-1] != K or x.device != wq.device:
+        raise ValueError(f"mxfp4_linear: input {tuple(x.shape)} on {x.device} does not match codes {tuple(wq.shape)} ([N, K / 2]) on "
+                         f"{wq.device}")
+    needs_x = x.requires_grad and torch.is_grad_enabled()
+    needs_w = weight is not None and weight.requires_grad and torch.is_grad_enabled()
+    if not (needs_x or needs_w) and _lib.plain(x) and forward_ad._current_level < 0:
+        y = _product_with(x if x.dim() == 2 else x.reshape(-1, K), wq, fwd_scale)       # nothing to differentiate
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+    if needs_x or needs_w:
+        if needs_x:
             if N % 128 or K % 128:
                 raise ValueError(f"the input gradient of mxfp4_linear needs dims that are multiples of 128, got {N} x {K}")
             if dgrad_scale is None:
                 raise ValueError("the input gradient of mxfp4_linear needs the scales of the transposed weight (dgrad_scale)")
-        if weight is not None and weight.requires_grad and (N % 8 or K % 8):
+        if needs_w and (N % 8 or K % 8):
             raise ValueError(f"the weight gradient of mxfp4_linear needs dims that are multiples of 8, got {N} x {K}")
     return _Mxfp4Linear.apply(x, weight, wq, fwd_scale, dgrad_scale)

@@ -57,7 +57,8 @@ def check_product(y, a, b):
 @pytest.mark.parametrize("M,N,K", [
     (1, 128, 256), (1, 1, 32), (1, 4096, 4096), (3, 130, 96), (16, 256, 160), (17, 384, 1024), (32, 100, 2080), (48, 1000, 512),
     (64, 129, 4096), (65, 128, 128), (128, 512, 1152), (129, 300, 640), (257, 1000, 800), (777, 1290, 416), (1024, 2048, 256), (513, 257, 32), (600, 3000, 1056),
-    (2305, 2440, 288), (4104, 1560, 384), (1300, 9000, 4096)])
+    (2305, 2440, 288), (4104, 1560, 384), (1300, 9000, 4096),
+    (100, 300, 14400), (130, 260, 7200), (33, 70, 9248), (20, 1111, 5984)])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_product(M, N, K, dt):
     aq, sa, a = operand(M, K, 1)
@@ -83,6 +84,25 @@ def test_product_of_strided_codes_and_nan_groups():
     bad[5] = True
     assert torch.equal(y.isnan(), bad)
     ops.check_status()
+
+
+@pytest.mark.parametrize("T,N,K,pad", [
+    (1, 128, 32, 0), (1, 1, 64, 0), (2, 300, 2080, 8), (5, 1000, 4128, 3), (16, 200, 1056, 0), (9, 4096, 14336, 0), (16, 131, 288, 1),
+    (3, 257, 40000, 0), (1, 6144, 4096, 0), (12, 40, 106496, 0), (1, 64, 110016, 0), (17, 300, 2080, 0), (90, 513, 800, 5)])
+def test_scoring_with_a_frozen_weight(T, N, K, pad):
+    """The quantiser and the product behind one call, inside one kernel for few rows: sums of K products in parts, in fp32."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    base = torch.randn(T, K + pad, generator=g, device="cuda").bfloat16()
+    x = base[:, pad:]
+    bq, sb, b = operand(N, K, 7)
+    y = m4.mxfp4_linear(x, None, bq, sb, None)
+    ops.check_status()
+    check_product(y, m4.mx4_dequantize(*m4.mx4_quantize_act(x), torch.float32).double(), b)
+    assert torch.equal(y, m4.mxfp4_linear(x, None, bq, sb, None))
+    assert torch.equal(m4.mxfp4_linear(x[None], None, bq, sb, None), y[None])
+    x[T - 1, K - 1] = float("inf")
+    y = m4.mxfp4_linear(x, None, bq, sb, None)
+    assert y[T - 1].isnan().all() and not y[:T - 1].isnan().any()
 
 
 @pytest.mark.parametrize("T,N,K", [(1, 256, 128), (100, 128, 384), (384, 512, 256), (256, 1152, 640)])
