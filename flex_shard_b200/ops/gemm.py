@@ -103,8 +103,8 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_t: bool = False, b_t: bool = Fal
     b = _rowmajor(b)
     if c is not None:
         assert c.shape == (M, N) and c.stride(1) == 1 and c.dtype in (torch.bfloat16, torch.float32)
-    if K % 8 != 0 or (a_t and M % 8 != 0) or (b_t and N % 8 != 0):
-        raise ValueError("gemm: K (and the contiguous dim of transposed operands) must be a multiple of 8")
+    if (K % 8 != 0 and not (a_t and b_t)) or (a_t and M % 8 != 0) or (b_t and N % 8 != 0):
+        raise ValueError("gemm: the contiguous dim of each operand (K, or M / N of a transposed one) must be a multiple of 8")
     lib = _lib.load()
     status = _lib.status_word(a.device)
     rc = lib.fsb_gemm_bf16(

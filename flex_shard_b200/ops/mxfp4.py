@@ -231,11 +231,6 @@ def gemm_mxfp4(aq, sfa, bq, sfb, *, out_dtype: torch.dtype = torch.bfloat16) -> 
     return out
 
 
-def _whole_octets(t: torch.Tensor) -> torch.Tensor:
-    """Rows padded with zeros to a multiple of 8, which the bf16 product over the rows needs."""
-    return t if t.shape[0] % 8 == 0 else torch.nn.functional.pad(t, (0, 0, 0, -t.shape[0] % 8))
-
-
 def _product_with(x2, wq, fwd_scale):
     """``[T, K]`` rows times the quantised weight: the forward pass of ``mxfp4_linear``."""
     T, K = x2.shape
@@ -293,8 +288,7 @@ class _Mxfp4Linear(torch.autograd.Function):
             gd = gd if gd in (torch.bfloat16, torch.float32) else torch.bfloat16
             if main is not None and main.dtype in (torch.float32, torch.bfloat16):
                 if T > 0:
-                    gemm(_whole_octets(dy2), _whole_octets(x2), a_t=True, b_t=True, out=main,
-                         accumulate=bool(getattr(weight, "main_grad_written", False)))
+                    gemm(dy2, x2, a_t=True, b_t=True, out=main, accumulate=bool(getattr(weight, "main_grad_written", False)))
                     weight.main_grad_written = True
             elif T == 0:
                 dw = torch.zeros(N, K, dtype=gd, device=x2.device)
@@ -304,7 +298,7 @@ class _Mxfp4Linear(torch.autograd.Function):
                 xq, sx = mx_quantize_rows(x2)
                 dw = gemm_mxfp8(dq, sd, xq, sx, a_t=True, b_t=True, out_dtype=gd)
             else:
-                dw = gemm(_whole_octets(dy2), _whole_octets(x2), a_t=True, b_t=True, out_dtype=gd)
+                dw = gemm(dy2, x2, a_t=True, b_t=True, out_dtype=gd)
         return dx, dw, None, None, None
 
 
