@@ -164,7 +164,7 @@ struct TopSmem {
   unsigned long long lists[MAX_PARTS * 32];       // sorted alternatives of the row's parts (in the first CTA; 0: none)
   unsigned long long best[32];                    // ... of this part, then of the row
   unsigned long long cand[CAP];
-  uint32_t groups[GROUPS];
+  alignas(16) uint32_t groups[GROUPS];
   float cmax[MAX_CHUNKS][THREADS];
   uint16_t work[MAX_CHUNKS * THREADS];
   uint32_t bound;
@@ -190,7 +190,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* from, int n,
 // logits), those above the bound are collected and those equal to it counted off from the lowest index; where even the former
 // do not fit, k maxima are taken one after the other.
 template <typename T, int THREADS>
-__device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at, float tmax, int cl,
+__device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at, float tmax, int cl_bits,
                                       int k, int lo, int hi, TopSmem<THREADS>& sm) {
   constexpr int L = Vec<T>::L, WARPS = THREADS / 32, PER = THREADS / GROUPS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -202,14 +202,19 @@ __device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, in
   if (tid < 32) sm.best[tid] = 0;
   if (tid < 4) sm.count[tid] = 0;
   __syncthreads();
-  if (tid < GROUPS) {
-    const uint32_t mine = sm.groups[tid];
+  {   // rank of group tid / PER, each of its threads counting over a part of the groups
+    constexpr int MANY = GROUPS / PER;
+    const int group = tid / PER, from = tid % PER * MANY;
+    const uint32_t mine = sm.groups[group];
     int rank = 0;
-#pragma unroll 16
-    for (int j = 0; j < GROUPS; ++j) {
-      const uint32_t o = sm.groups[j];
-      rank += o > mine || (o == mine && j < tid) ? 1 : 0;
+#pragma unroll
+    for (int j = from; j < from + MANY; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&sm.groups[j]);
+      rank += (o.x > mine || (o.x == mine && j < group)) + (o.y > mine || (o.y == mine && j + 1 < group)) +
+              (o.z > mine || (o.z == mine && j + 2 < group)) + (o.w > mine || (o.w == mine && j + 3 < group));
     }
+#pragma unroll
+    for (int o = PER / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
     if (rank == k - 1) sm.bound = mine;
   }
   __syncthreads();
@@ -219,27 +224,31 @@ __device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, in
   auto collect = [&](uint32_t least, int& chunks, int& count) {
     const float lf = key_value(least);
     auto offer = [&](float f, int at) {
-      if (!(f < lf) && value_key(f) >= least) {
+      if (value_key(f) >= least) {
         const int slot = atomicAdd(&count, 1);
         if (slot < CAP) sm.cand[slot] = order_key(f, at);
       }
     };
     if (own >= least) {
       if (edge_at >= 0) offer(edge, edge_at);
-      const int n = first_vec + tid < end_vec ? (end_vec - first_vec - tid + THREADS - 1) / THREADS : 0;
-      for (int ch = 0; ch * cl < n; ++ch)
-        if (value_key(sm.cmax[ch][tid]) >= least) sm.work[atomicAdd(&chunks, 1)] = static_cast<uint16_t>(ch * THREADS + tid);
+      uint32_t some = 0;
+#pragma unroll
+      for (int ch = 0; ch < MAX_CHUNKS; ++ch) some |= (value_key(sm.cmax[ch][tid]) >= least ? 1u : 0u) << ch;
+      for (; some != 0; some &= some - 1) sm.work[atomicAdd(&chunks, 1)] = static_cast<uint16_t>((__ffs(some) - 1) * THREADS + tid);
     }
     __syncthreads();
-    const int units = chunks * cl;
+    const int units = chunks << cl_bits;
     for (int i = tid; i < units; i += THREADS) {
-      const int item = i / cl, w = sm.work[item];
-      const int vec = first_vec + w % THREADS + (w / THREADS * cl + i - item * cl) * THREADS;
-      if (vec >= end_vec) continue;
+      const int w = sm.work[i >> cl_bits], j = (w / THREADS << cl_bits) + (i & ((1 << cl_bits) - 1));
+      const int vec = first_vec + w % THREADS + j * THREADS;
+      if (vec >= end_vec) continue;                   // the last chunk of a thread may be short, or there may be none
+      const int at = head + vec * L;
       float f[L];
-      Vec<T>::unpack(*reinterpret_cast<const uint4*>(r + head + static_cast<long long>(vec) * L), f);
+      Vec<T>::unpack(*reinterpret_cast<const uint4*>(r + at), f);
+      uint32_t some = 0;
 #pragma unroll
-      for (int e = 0; e < L; ++e) offer(f[e], head + vec * L + e);
+      for (int e = 0; e < L; ++e) some |= (f[e] < lf ? 0u : 1u) << e;     // NaN too
+      for (; some != 0; some &= some - 1) offer(to_f(r[at + __ffs(some) - 1]), at + __ffs(some) - 1);
     }
     __syncthreads();
   };
@@ -336,7 +345,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   const int per = (span.nvec + parts - 1) / parts;
   const int first_vec = min(part * per, span.nvec), end_vec = min(first_vec + per, span.nvec);
   const int n = (end_vec - first_vec + THREADS - 1) / THREADS;      // vectors of a thread
-  const int cl = max(4, ((n + MAX_CHUNKS - 1) / MAX_CHUNKS + 3) / 4 * 4);
+  const int cl_bits = max(2, 32 - __clz((n + MAX_CHUNKS - 1) / MAX_CHUNKS - 1));   // a chunk: 2^cl_bits vectors, 4 or more
   Sums a{floor_, 0.f, 0.f};
   float tmax = -INFINITY, cmax = -INFINITY;
   auto take = [&](const uint4& v) {
@@ -364,7 +373,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     for (int q = 0; q < 4; ++q) take(v[q]);
     if constexpr (TOP) {
       in_chunk += 4;
-      if (in_chunk == cl) {
+      if (in_chunk == 1 << cl_bits) {
         ts.cmax[chunk++][tid] = cmax;
         tmax = max_nan(tmax, cmax);
         cmax = -INFINITY;
@@ -373,8 +382,11 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     }
   }
   if constexpr (TOP) {
-    if (in_chunk) ts.cmax[chunk][tid] = cmax;
     tmax = max_nan(tmax, cmax);
+    for (; chunk < MAX_CHUNKS; ++chunk) {
+      ts.cmax[chunk][tid] = cmax;
+      cmax = -INFINITY;
+    }
   }
   // the elements before and after the vectors, one a thread
   const int edges = (part == 0 ? span.head : 0) + (part == parts - 1 ? span.tail : 0);
@@ -422,7 +434,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   Sums all = combine(sm.warp, WARPS);
   if constexpr (TOP) {
     const int lo = part == 0 ? 0 : span.head + first_vec * L, hi = part == parts - 1 ? V : span.head + end_vec * L;
-    part_top<T, THREADS>(r, first_vec, end_vec, span.head, edge, edge_at, tmax, cl, k, lo, hi, ts);
+    part_top<T, THREADS>(r, first_vec, end_vec, span.head, edge, edge_at, tmax, cl_bits, k, lo, hi, ts);
   }
   if (parts > 1) {
     cluster_wait();                                  // every CTA of the cluster has started: the first one's memory is there
