@@ -586,14 +586,18 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ targe
   }
 }
 
-constexpr int SMALL_V = 8192, LARGE = 256;
+constexpr int SMALL = 128, LARGE = 256;     // threads of a CTA
 
-// CTAs of a row: enough to fill the SMs twice, but at least 4096 elements each.
-int row_parts(long long T, int V) {
+// CTAs of a row: as many as `places` allow, with 4096 elements or more each.
+int row_parts(long long T, int V, int places) {
   int parts = 1;
-  while (parts < MAX_PARTS && T * parts * 2 <= 296 && V / (parts * 2) >= 4096) parts *= 2;
+  while (parts < MAX_PARTS && T * parts * 2 <= places && V / (parts * 2) >= 4096) parts *= 2;
   return parts;
 }
+// Small CTAs, of which an SM holds ten, hide the ends of short rows; a long row, or the only one an SM has, streams faster into a
+// large one. Forward with 8 alternatives, 128 / 256 threads: 20000 x 2000 bf16 95 / 174 us, 6000 x 12000 47 / 72, 8192 x 32000
+// 122 / 143, 4096 x 64000 104 / 113, 4096 x 128256 199 / 199, 1500 x 50021 fp32 63 / 59, 148 x 128256 30 / 19.
+bool small_ctas(long long ctas, int V, int size) { return V <= 8192 || (static_cast<long long>(V) * size <= 128 * 1024 && ctas >= 592); }
 
 inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH; }
 }  // namespace
@@ -606,12 +610,14 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
   if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2) return FSB_ERR_BAD_ARG;
   if (T > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   if (T == 0) return FSB_OK;
-  const int parts = row_parts(T, V);
+  // One CTA an SM is enough: with alternatives the parts' exchange costs more than it gains (74 x 128256, 2 / 4 / 8 parts: 10.3,
+  // 12.7, 19.8 us; 7 rows 8 parts 9.1), without it is even (7.3, 8.1, 8.3).
+  const int parts = row_parts(T, V, 148);
   if (T * parts > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(T * parts), 1, 1);
-  const bool small = V <= SMALL_V;
-  cfg.blockDim = dim3(small ? 128 : LARGE, 1, 1);
+  const bool small = small_ctas(T * parts, V, kind == 2 ? 4 : 2);
+  cfg.blockDim = dim3(small ? SMALL : LARGE, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -622,8 +628,8 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
   cfg.numAttrs = parts > 1 ? 1 : 0;
   auto run = [&](auto* p) {
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    auto kernel = k > 0 ? (small ? logprobs_kernel<E, true, 128> : logprobs_kernel<E, true, LARGE>)
-                        : (small ? logprobs_kernel<E, false, 128> : logprobs_kernel<E, false, LARGE>);
+    auto kernel = k > 0 ? (small ? logprobs_kernel<E, true, SMALL> : logprobs_kernel<E, true, LARGE>)
+                        : (small ? logprobs_kernel<E, false, SMALL> : logprobs_kernel<E, false, LARGE>);
     const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p, target, V, ld, inv_t, k, ignore_index, parts, logprob, entropy,
                                                static_cast<float2*>(stats), top_lp, top);
     const int rc = ok();   // also clears the error of a launch that failed
@@ -644,11 +650,12 @@ FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* tar
   if (T == 0) return FSB_OK;
   auto run = [&](auto* p) {
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    const dim3 grid(static_cast<unsigned>(T), row_parts(T, V));
-    auto kernel = V <= SMALL_V ? logprobs_bwd_kernel<E, 128> : logprobs_bwd_kernel<E, LARGE>;
-    kernel<<<grid, V <= SMALL_V ? 128 : LARGE, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
-                                                            static_cast<const float2*>(stats), entropy, glp, gh, gtop,
-                                                            static_cast<E*>(dx), ldd);
+    const dim3 grid(static_cast<unsigned>(T), row_parts(T, V, 592));     // the parts have nothing to exchange
+    const bool small = V <= 8192;     // longer rows: even (8192 x 32000 187 / 189 us, 4096 x 128256 362 / 350)
+    auto kernel = small ? logprobs_bwd_kernel<E, SMALL> : logprobs_bwd_kernel<E, LARGE>;
+    kernel<<<grid, small ? SMALL : LARGE, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
+                                                       static_cast<const float2*>(stats), entropy, glp, gh, gtop,
+                                                       static_cast<E*>(dx), ldd);
     return ok();
   };
   if (kind == 0) return run(static_cast<const __nv_bfloat16*>(x));
