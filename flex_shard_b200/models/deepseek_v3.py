@@ -23,6 +23,7 @@ from ..ops import elementwise as ew
 from ..ops import moe as moe_ops
 from ..ops.embedding import TokenEmbedding
 from ..ops.gemm import linear
+from ..ops.logprobs import TokenLogprobs, token_logprobs
 from ..ops.mla import mla_operands
 
 
@@ -275,6 +276,13 @@ class DeepSeekV3(nn.Module):
 
     def loss(self, tokens, targets, loss_is_root: bool = True, positions=None):
         return ew.cross_entropy(self(tokens, positions), targets.reshape(-1), unit_grad=loss_is_root)
+
+    def token_logprobs(self, tokens, targets, positions=None, temperature: float = 1.0, top_k: int = 0, ignore_index: int = -100):
+        """Log probability of every token of ``targets`` (shape of ``tokens``) with the entropy and the ``top_k`` likeliest
+        alternatives at its position (``ops.logprobs.token_logprobs``)."""
+        out = token_logprobs(self(tokens, positions), targets.reshape(-1), temperature=temperature, top_k=top_k,
+                             ignore_index=ignore_index)
+        return TokenLogprobs(*(t.view(*targets.shape, *t.shape[1:]) for t in out))
 
     def moe_layers(self):
         return [b.moe for b in self.layers if hasattr(b, "moe")]

@@ -20,6 +20,7 @@ from ..ops import elementwise as ew
 from ..ops.attention import qkv_attention
 from ..ops.embedding import TokenEmbedding
 from ..ops.gemm import linear
+from ..ops.logprobs import TokenLogprobs, token_logprobs
 
 
 @dataclass
@@ -142,6 +143,14 @@ class Llama(nn.Module):
         incoming gradient is taken to be 1, which saves a pass over the logits)."""
         logits = self(tokens)  # through __call__, so that root-level bucket hooks run
         return ew.cross_entropy(logits, targets.reshape(-1), unit_grad=loss_is_root)
+
+
+    def token_logprobs(self, tokens, targets, temperature: float = 1.0, top_k: int = 0, ignore_index: int = -100):
+        """Log probability of every token of ``targets`` (shape of ``tokens``) with the entropy and the ``top_k`` likeliest
+        alternatives at its position (``ops.logprobs.token_logprobs``): policy gradients, scoring, distillation."""
+        logits = self(tokens)
+        out = token_logprobs(logits, targets.reshape(-1), temperature=temperature, top_k=top_k, ignore_index=ignore_index)
+        return TokenLogprobs(*(t.view(*targets.shape, *t.shape[1:]) for t in out))
 
 
 def llama_quantized_buckets(model: Llama, mesh=None, kind: str = "fp8", mp_policy=None):

@@ -10,6 +10,7 @@ from .linear import (
     convert_to_flex_shard_mxfp4_blockwise_linear,
     convert_to_flex_shard_mxfp8_blockwise_linear,
     convert_to_flex_shard_prequantized_linear,
+    freeze_mxfp4_weights_,
 )
 from .weight import (
     BlockwiseFp8Weight,

@@ -215,6 +215,30 @@ class FlexShardMxfp4BlockwiseLinear(FlexShardPrequantizedLinear):
         return mxfp4_linear(x, None if isinstance(w, BlockwiseMxfp4Weight) else w, q, fwd, dgrad)
 
 
+def freeze_mxfp4_weights_(module: nn.Module, patterns) -> nn.Module:
+    """Replaces the matrices whose dotted names match one of ``patterns`` (``fnmatch``, as in ``BucketSpec``) by their 4-bit
+    payloads, for scoring with a frozen model (a teacher, a reference policy): every ``linear`` on such a weight runs the
+    4-bit product, gradients pass through to its input, the weight takes none. For the decoders of this library, for
+    instance, ``["layers.*.w*", "head.output"]``. The module must not be sharded; other matrices than those that go through
+    ``linear`` (an embedding, a router) must not match."""
+    from fnmatch import fnmatchcase
+
+    from ..flex_shard import FlexShardModule
+
+    if any(isinstance(m, FlexShardModule) for m in module.modules()):
+        raise ValueError("freeze_mxfp4_weights_ works on modules that are not sharded")
+    chosen = [(f"{prefix}.{name}" if prefix else name, m, name, p) for prefix, m in module.named_modules()
+              for name, p in m.named_parameters(recurse=False) if any(fnmatchcase(f"{prefix}.{name}" if prefix else name, q) for q in patterns)]
+    if not chosen:
+        raise ValueError(f"no parameter matches {list(patterns)}")
+    for fqn, _, _, p in chosen:
+        if isinstance(p, BlockwiseQuantWeight) or p.dim() != 2 or p.shape[1] % 32:
+            raise ValueError(f"{fqn}: {type(p).__name__} {tuple(p.shape)} is not a matrix whose columns are a multiple of 32")
+    for _, m, name, p in chosen:
+        setattr(m, name, nn.Parameter(BlockwiseMxfp4Weight.from_float(p), requires_grad=False))
+    return module
+
+
 def _eligible(child) -> bool:
     return (isinstance(child, nn.Linear) and child.bias is None and child.in_features % 128 == 0
             and child.out_features % 128 == 0)
