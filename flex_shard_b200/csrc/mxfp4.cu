@@ -1172,7 +1172,7 @@ FSB_API int fsb_gemm_mxfp4(const void* aq, const void* sfa, const void* bq, cons
 }
 
 // d[M, N] = Q(x) B^T for bf16 x [M, K] with row stride ldx: the quantiser and the product, in one launch for up to 16 rows.
-// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes on a 16-byte boundary.
+// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes on a 16-byte boundary; null: FSB_ERR_TOO_LARGE where it takes two.
 FSB_API int fsb_mxfp4_linear(const void* x, long long ldx, const void* bq, long long ldb, const void* sfb, void* d, long long ldd,
                              void* scratch, int M, int N, int K, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || ldb % 16 != 0) return FSB_ERR_BAD_ARG;
@@ -1182,7 +1182,8 @@ FSB_API int fsb_mxfp4_linear(const void* x, long long ldx, const void* bq, long 
     const int rc = launch_few(x, bq, sfb, a, ldx, ldb, stream);
     if (rc != FSB_ERR_TOO_LARGE) return rc;
   }
-  if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15)) return FSB_ERR_BAD_ARG;
+  if (scratch == nullptr) return FSB_ERR_TOO_LARGE;
+  if (reinterpret_cast<uintptr_t>(scratch) & 15) return FSB_ERR_BAD_ARG;
   uint8_t* q = static_cast<uint8_t*>(scratch);
   uint8_t* sf = q + static_cast<long long>(M) * (K / 2);      // K / 2 is a multiple of 16
   const int rc = fsb_mx4_quant_act(x, q, sf, M, K, ldx, stream);

@@ -237,23 +237,34 @@ def _product_with(x2, wq, fwd_scale):
     N = wq.shape[0]
     if not x2.is_cuda:
         return gemm_mxfp4(*mx4_quantize_act(x2), wq, fwd_scale)
-    out = torch.empty(T, N, dtype=torch.bfloat16, device=x2.device)
+    out = x2.new_empty(T, N)
     if T == 0 or N == 0:
         return out
     _ensure()
-    if x2.stride(1) != 1:
+    ldx, unit = x2.stride()
+    if unit != 1:
         x2 = x2.contiguous()
-    if wq.stride(1) != 1 or wq.stride(0) % 16 or wq.data_ptr() % 16:
+        ldx = K
+    ldw, unit = wq.stride()
+    if unit != 1 or ldw % 16 or wq.data_ptr() % 16:
         wq = wq.contiguous()
+        ldw = K // 2
     if fwd_scale.data_ptr() % 16:
         fwd_scale = fwd_scale.clone()
-    scratch = torch.empty(T * (K // 2) + blocked_scale_numel(T, K), dtype=torch.uint8, device=x2.device)   # codes, scales
+    linear = _lib.load().fsb_mxfp4_linear
+    status = _lib.status_word(x2.device).data_ptr()
+    rc = _lib.TOO_LARGE
     with _lib.device_of(x2):
-        rc = _lib.load().fsb_mxfp4_linear(x2.data_ptr(), x2.stride(0), wq.data_ptr(), wq.stride(0), fwd_scale.data_ptr(),
-                                          out.data_ptr(), N, scratch.data_ptr(), T, N, K,
-                                          _lib.status_word(x2.device).data_ptr(), _lib.stream_ptr(x2.device))
+        stream = _lib.stream_ptr(x2.device)
+        if T <= 4:      # mostly quantised inside the product, which needs no scratch
+            rc = linear(x2.data_ptr(), ldx, wq.data_ptr(), ldw, fwd_scale.data_ptr(), out.data_ptr(), N, None, T, N, K, status, stream)
+        if rc == _lib.TOO_LARGE:
+            scratch = torch.empty(T * (K // 2) + blocked_scale_numel(T, K), dtype=torch.uint8, device=x2.device)  # codes, scales
+            rc = linear(x2.data_ptr(), ldx, wq.data_ptr(), ldw, fwd_scale.data_ptr(), out.data_ptr(), N, scratch.data_ptr(), T, N, K,
+                        status, stream)
+            count_launch()
     _lib.check(rc, "fsb_mxfp4_linear")
-    count_launch(2)
+    count_launch()
     return out
 
 
