@@ -2,8 +2,8 @@
 (``csrc/logprobs.cu``). The counterpart of ``cross_entropy`` where a value per token is wanted: policy gradients,
 distillation on a teacher's alternatives, scoring.
 
-CPU tensors, and tensors that a kernel cannot be given (batched gradients, ``torch.func`` transforms, forward-mode
-derivatives), take a PyTorch restatement.
+CPU tensors take a PyTorch restatement of the same arithmetic, and so do ``torch.func`` transforms, forward-mode derivatives and
+batched gradients.
 """
 from __future__ import annotations
 
@@ -55,7 +55,8 @@ def _restatement(x, target, temperature, k, ignore_index):
     xf = x.float()
     lp = torch.log_softmax((xf - xf.detach().amax(-1, keepdim=True)) / temperature, -1)
     at = torch.where(valid, target, 0)
-    logprob = torch.where(valid, lp.gather(1, at[:, None]).squeeze(1), torch.where(live, torch.nan, 0.0))
+    # a target outside the vocabulary makes its row's value and gradient NaN
+    logprob = torch.where(live, lp.gather(1, at[:, None]).squeeze(1) * torch.where(live & ~valid, torch.nan, 1.0), 0.0)
     # 0 log 0 counts as 0; a NaN (no distribution) stays one
     p = lp.exp()
     plogp = torch.where(p == 0, 0.0, p * torch.where(p == 0, 0.0, lp))
@@ -74,21 +75,31 @@ def _restated_gradient(x, target, top, stats, entropy, temperature, ignore_index
     p = lp.exp()
     cols = torch.arange(V, device=x.device)
     dz = torch.zeros((), device=x.device)
+    wanted = torch.zeros((), dtype=torch.bool, device=x.device)
     if glp is not None:
         nan = torch.where(live & ~valid, torch.nan, 0.0)[:, None]
         dz = dz + glp[:, None] * ((cols == torch.where(valid, target, 0)[:, None]).float() - p + nan)
+        wanted = wanted | (glp != 0)
     if gh is not None:
         dz = dz - gh[:, None] * torch.where(p == 0, 0.0, p * (torch.where(p == 0, 0.0, lp) + entropy[:, None]))
+        wanted = wanted | (gh != 0)
     if gtop is not None:
         for i in range(top.shape[1]):
             dz = dz + gtop[:, i, None] * ((cols == top[:, i, None]).float() - p)
-    return (torch.where(live[:, None], dz, 0.0) / temperature).to(x.dtype)
+            wanted = wanted | (gtop[:, i] != 0)
+    return (torch.where((live & wanted)[:, None], dz, 0.0) / temperature).to(x.dtype)
 
 
 def _forward(x, target, temperature, k, ignore_index, stats):
-    """``stats`` [T, 2] takes the numbers of a row that the gradient starts from (``None``: not wanted)."""
-    _ensure()
+    """``stats`` [T, 2] takes the numbers of a row that the gradient starts from, the largest logit and the logarithm of the
+    sum relative to it (``None``: not wanted)."""
     T, V = x.shape
+    if not x.is_cuda:
+        if stats is not None:
+            m = x.float().amax(-1, keepdim=True)
+            stats.copy_(torch.cat([m, ((x.float() - m) / temperature).exp().sum(-1, keepdim=True).log()], -1))
+        return _restatement(x, target, temperature, k, ignore_index)
+    _ensure()
     dev = x.device
     logprob = torch.empty(T, dtype=torch.float32, device=dev)
     entropy = torch.empty(T, dtype=torch.float32, device=dev)
@@ -127,7 +138,7 @@ class _TokenLogprobs(torch.autograd.Function):
         given = [g for g in (glp, gh, gtop) if g is not None]
         if not given:
             return None, None, None, None, None
-        if not _lib.plain(*given):
+        if not x.is_cuda or not _lib.plain(*given):
             return _restated_gradient(x, target, top, stats, entropy, temperature, ignore_index, glp, gh, gtop), None, None, None, None
         glp, gh, gtop = (None if g is None else g.float().contiguous() for g in (glp, gh, gtop))
         # rows of the gradient start as far into 16 bytes as the logits' rows do, so that both move in whole vectors
@@ -182,7 +193,7 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, *, temperature: f
         x, t = x.reshape(-1, V), t.reshape(-1)
     if t.dtype != torch.int64:
         t = t.long()
-    if x.is_cuda and _lib.plain(logits, target) and forward_ad._current_level < 0:
+    if _lib.plain(logits, target) and forward_ad._current_level < 0:
         if V > 1 and x.stride(1) != 1:
             x = x.contiguous()
         if not t.is_contiguous():

@@ -61,6 +61,11 @@ def _check_operand(q: torch.Tensor, scales: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what}: scales must be at least {need} contiguous uint8 bytes in block layout on the codes' device")
 
 
+def _ld(t: torch.Tensor) -> int:
+    """Row stride in elements; a single row has any stride."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 # --------------------------------------------------------------------------- restatement
 def _exponent(amax: torch.Tensor) -> torch.Tensor:
     bits = amax.float().contiguous().view(torch.int32)
@@ -167,12 +172,12 @@ def mx4_quantize_weight_operands(w: torch.Tensor):
 def _expand(q: torch.Tensor, scales, dtype: torch.dtype) -> torch.Tensor:
     _ensure()
     T, K = q.shape[0], 2 * q.shape[1]
-    if q.stride(1) != 1 or q.stride(0) % 4 or q.data_ptr() % 4:
-        q = q.contiguous()
+    if q.stride(1) != 1 or _ld(q) % 4 or q.data_ptr() % 4:
+        q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty(T, K, dtype=dtype, device=q.device)
     with _lib.device_of(q):
         rc = _lib.load().fsb_mx4_expand(q.data_ptr(), scales.data_ptr() if scales is not None else None, out.data_ptr(), T, K,
-                                        q.stride(0), _KINDS[dtype], _lib.stream_ptr(q.device))
+                                        _ld(q), _KINDS[dtype], _lib.stream_ptr(q.device))
     _lib.check(rc, "fsb_mx4_expand")
     count_launch(int(T > 0))
     return out
@@ -219,12 +224,13 @@ def gemm_mxfp4(aq, sfa, bq, sfb, *, out_dtype: torch.dtype = torch.bfloat16) -> 
     if M == 0 or N == 0:
         return out
     _ensure()
-    aq, bq = (t if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0 else t.contiguous() for t in (aq, bq))
+    aq, bq = (t if t.stride(1) == 1 and _ld(t) % 16 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+              for t in (aq, bq))
     sfa, sfb = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (sfa, sfb))
     status = _lib.status_word(aq.device)
     with _lib.device_of(aq):
         rc = _lib.load().fsb_gemm_mxfp4(aq.data_ptr(), sfa.data_ptr(), bq.data_ptr(), sfb.data_ptr(), out.data_ptr(), M, N, K,
-                                        aq.stride(0), bq.stride(0), out.stride(0), int(out_dtype == torch.float32),
+                                        _ld(aq), _ld(bq), N, int(out_dtype == torch.float32),
                                         status.data_ptr(), _lib.stream_ptr(aq.device))
     _lib.check(rc, "fsb_gemm_mxfp4")
     count_launch()
@@ -241,13 +247,11 @@ def _product_with(x2, wq, fwd_scale):
     if T == 0 or N == 0:
         return out
     _ensure()
-    ldx, unit = x2.stride()
-    if unit != 1:
+    if x2.stride(1) != 1:
         x2 = x2.contiguous()
-        ldx = K
-    ldw, unit = wq.stride()
-    if unit != 1 or ldw % 16 or wq.data_ptr() % 16:
-        wq = wq.contiguous()
+    ldx, ldw = _ld(x2), _ld(wq)
+    if wq.stride(1) != 1 or ldw % 16 or wq.data_ptr() % 16:
+        wq = wq.clone(memory_format=torch.contiguous_format)
         ldw = K // 2
     if fwd_scale.data_ptr() % 16:
         fwd_scale = fwd_scale.clone()

@@ -71,6 +71,28 @@ def test_rows_without_a_distribution_and_odd_targets():
     assert out.logprob[5] == 0 and out.entropy[5] == 0 and out.top_index[5].tolist() == [-1, -1]
 
 
+def test_gradients_of_odd_rows():
+    """A row whose gradients are all 0 has none, whatever its logits; a target outside the vocabulary makes its row NaN."""
+    x, t = rows(4, 20, torch.float32)
+    x[0], t[1], t[3] = math.nan, 25, -100
+    x.requires_grad_()
+    out = token_logprobs(x, t, top_k=2)
+    (dx,) = torch.autograd.grad(out.logprob, x, torch.tensor([0.0, 1.0, 1.0, 1.0]))
+    assert not dx[0].any() and dx[1].isnan().all() and dx[2].isfinite().all() and dx[2].any() and not dx[3].any()
+    with pytest.raises(RuntimeError):
+        (d,) = torch.autograd.grad(token_logprobs(x, t).entropy[2], x, create_graph=True)
+        d.sum().backward()
+
+
+def test_transforms_and_forward_derivatives_take_the_restatement():
+    x, t = rows(3, 11, torch.float32)
+    f = lambda z: token_logprobs(z, t, top_k=2).logprob.sum()  # noqa: E731
+    want = gradient(x, t, 1.0, 2, torch.ones(3), torch.zeros(3), torch.zeros(3, 2))[0]
+    torch.testing.assert_close(torch.func.grad(f)(x).double(), want, rtol=0, atol=1e-5)
+    v = torch.randn(3, 11)
+    torch.testing.assert_close(torch.func.jvp(f, (x,), (v,))[1].double(), (want * v).sum(), rtol=0, atol=1e-4)
+
+
 def test_leading_axes_and_equal_logits():
     x = torch.zeros(2, 3, 40)
     x[..., 7] = -0.0

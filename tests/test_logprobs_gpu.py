@@ -197,3 +197,28 @@ def test_results_do_not_change_from_call_to_call():
     first = token_logprobs(x, t, top_k=20)
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(first, token_logprobs(x, t, top_k=20)))
+
+
+def test_rows_far_apart():
+    """Row offsets that pass 32 bits (a cache of logits, of which every millionth row is scored)."""
+    ld, V = 1_100_000_008, 5001
+    base = torch.empty(2 * ld + V + 3, dtype=BF, device="cuda")
+    x = base[3:].as_strided((3, V), (ld, 1))
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x.copy_(torch.randn(3, V, generator=g, device="cuda") * 3)
+    check(x, torch.tensor([5, 5000, 0], device="cuda"), 1.0, 4)
+
+
+@pytest.mark.parametrize("V,period,held,dtype", [(40000, 2048, 992, BF), (8000, 1024, 496, BF), (40000, 1024, 496, FP), (120000, 2048, 992, HF)])
+def test_large_logits_that_few_threads_hold(V, period, held, dtype):
+    """Rows whose large logits all fall to less than half of the threads, so that neither all above the bound on the
+    alternatives nor all equal to it fit the candidates; with many equal ones, and with none."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    where = torch.arange(V, device="cuda") % period < held
+    x = torch.zeros(3, V, device="cuda")
+    x[0, where] = 1 + torch.rand(int(where.sum()), generator=g, device="cuda")
+    x[1, where] = 2.0
+    x[2] = torch.randn(V, generator=g, device="cuda") - 20
+    x[2, where] += 30
+    for k in (31, 32):
+        check(x.to(dtype), torch.tensor([3, V - 1, 7], device="cuda"), 1.0, k)

@@ -126,6 +126,63 @@ def test_linear_and_its_gradients(T, N, K):
         check_product(dw, dy.double().t(), x.detach().double().t())
 
 
+def test_sizes_that_pass_32_bits():
+    """Codes, inputs and outputs whose last rows lie past 2^31 elements."""
+    T, K, N = 1_049_700, 2048, 2064
+    base = torch.randn(64, K, device="cuda").bfloat16()
+    x = base.repeat(T // 64 + 1, 1)[:T]
+    same = torch.arange(T - 100, T, device="cuda") % 64     # rows of the base that the last rows repeat
+    q, s = m4.mx4_quantize_act(x)
+    q_ref, s_ref = m4.mx4_quantize_act(base)
+    assert torch.equal(q[-100:], q_ref[same])
+    bq, sb, b = operand(N, K, 8)
+    y = m4.gemm_mxfp4(q, s, bq, sb)
+    ops.check_status()
+    check_product(y[-100:], m4.mx4_dequantize(q_ref, s_ref, torch.float32).double()[same], b)
+    del y
+    assert torch.equal(m4.mx4_dequantize(q, s)[-100:], m4.mx4_dequantize(q_ref, s_ref)[same])
+
+
+def test_a_single_row_of_any_stride():
+    K, N = 256, 40
+    bq, sb, b = operand(N, K, 9)
+    aq, sa, a = operand(1, K, 10)
+    odd = torch.zeros(K // 2, 3, dtype=torch.uint8, device="cuda")
+    odd[:, 1] = aq[0]
+    row = odd[:, 1:2].t()                                   # [1, K / 2] with strides (1, 3)
+    check_product(m4.gemm_mxfp4(row, sa, bq, sb), a, b)
+    check_product(m4.gemm_mxfp4(aq.as_strided((1, K // 2), (7, 1)), sa, bq, sb), a, b)
+    assert torch.equal(m4.mx4_dequantize(row, sa), m4.mx4_dequantize(aq, sa))
+
+
+@pytest.mark.parametrize("grad_bucket", [False, True])
+def test_sharded_layers_train_like_unsharded_ones(grad_bucket):
+    """The gradients of a sharded stack (written into the bucket where it offers its rows) and of the plain one; an fp32 bucket
+    takes them unrounded, the plain weight in bf16."""
+    from flex_shard_b200 import BucketSpec, MixedPrecisionPolicy, flex_shard
+    from flex_shard_b200.placements.shard import shard_placement_fn
+
+    def net():
+        torch.manual_seed(0)
+        m = torch.nn.Sequential(FlexShardMxfp4BlockwiseLinear(256, 384, device="cuda"), FlexShardMxfp4BlockwiseLinear(384, 128, device="cuda"))
+        for p in m.parameters():
+            torch.nn.init.normal_(p, std=0.05)
+        return m
+
+    x, dy = torch.randn(200, 256, device="cuda").bfloat16(), torch.randn(200, 128, device="cuda").bfloat16()
+    plain, sharded = net(), net()
+    flex_shard(sharded, [BucketSpec(["*"], mp_policy=MixedPrecisionPolicy(param_dtype=torch.bfloat16, reduce_dtype=torch.float32),
+                                    placement_fn=shard_placement_fn(0, grad_bucket=grad_bucket))])
+    y, z = plain(x), sharded(x)
+    assert torch.equal(y, z)
+    y.backward(dy)
+    z.backward(dy)
+    ops.check_status()
+    for a, b in zip(plain.parameters(), sharded.parameters()):
+        ga, gb = a.grad.double(), b.grad.double().view(a.shape)
+        assert gb.any() and ((ga - gb).abs() <= gb.abs() * 2.0 ** -7).all()     # one rounding to bf16 on either side
+
+
 def test_layer_trains_and_scores_in_a_captured_graph():
     torch.manual_seed(0)
     layer = FlexShardMxfp4BlockwiseLinear(256, 512, device="cuda")
