@@ -239,6 +239,7 @@ __device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, in
     __syncthreads();
     const int units = chunks << cl_bits;
     for (int i = tid; i < units; i += THREADS) {
+      if (*static_cast<volatile int*>(&count) > CAP) break;   // too many already: masked logits, for the most part
       const int w = sm.work[i >> cl_bits], j = (w / THREADS << cl_bits) + (i & ((1 << cl_bits) - 1));
       const int vec = first_vec + w % THREADS + j * THREADS;
       if (vec >= end_vec) continue;                   // the last chunk of a thread may be short, or there may be none
