@@ -190,7 +190,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* from, int n,
 // logits), those above the bound are collected and those equal to it counted off from the lowest index; where even the former
 // do not fit, k maxima are taken one after the other.
 template <typename T, int THREADS>
-__device__ __noinline__ void part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at, float tmax, int cl_bits,
+__device__ __forceinline__ void part_top(const T* r, int first_vec, int end_vec, int head, float edge, int edge_at, float tmax, int cl_bits,
                                       int k, int lo, int hi, TopSmem<THREADS>& sm) {
   constexpr int L = Vec<T>::L, WARPS = THREADS / 32, PER = THREADS / GROUPS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
