@@ -3,7 +3,8 @@
     python -m flex_shard_b200.utils.kernel_cases <case> [--iters N]
 
 Cases: gemm_fwd, gemm_dgrad, gemm_wgrad, attn_fwd, attn_bwd, attn_bwd_ordered, adamw, rmsnorm, rmsnorm_bwd, swiglu, cross_entropy,
-newton_schulz, newton_schulz_batched, fp8_quant, fp8_gemm, mxfp8_gemm, allgather_gemm, segment_cast. Each prints one JSON line with the CUDA-event time (median of
+newton_schulz, newton_schulz_batched, fp8_quant, fp8_gemm, mxfp8_gemm, mxfp4_gemm, mxfp4_quant,
+token_logprobs, allgather_gemm, segment_cast. Each prints one JSON line with the CUDA-event time (median of
 ``iters`` launches after 3 warm-up launches, L2 flushed between launches by writing a 256 MB buffer)
 and the achieved FLOP/s or bytes/s. Inputs are a few hundred MB, larger than the 126 MB L2, so DRAM
 counters of a profiler capture of the same command stay meaningful.
@@ -201,6 +202,41 @@ def main():
                        max_abs_diff_vs_cublaslt=float((ref.float() - ours.float()).abs().max()))
         except Exception as ex:  # noqa: BLE001
             out.update(cublaslt="unavailable: " + str(ex).split("\n")[0][:120])
+    elif args.case == "mxfp4_gemm":
+        from flex_shard_b200.ops import mxfp4 as m4
+
+        M, N, K = 8192, 28672, 4096
+        xq, sx = m4.mx4_quantize_act(torch.randn(M, K, device=dev).bfloat16())
+        wq, _, fwd, _ = m4.mx4_quantize_weight_operands(torch.randn(N, K, device=dev).bfloat16())
+        ms = _time(lambda: m4.gemm_mxfp4(xq, sx, wq, fwd), args.iters)
+        x1 = torch.randn(1, K, device=dev).bfloat16()
+        ms_1 = _time(lambda: m4.mxfp4_linear(x1, None, wq, fwd, None), args.iters)
+        out.update(M=M, N=N, K=K, ms=ms, tflops=2.0 * M * N * K / ms / 1e9, one_row_ms=ms_1, one_row_gbs=N * K / 2 / ms_1 / 1e6)
+    elif args.case == "mxfp4_quant":
+        from flex_shard_b200.ops import mxfp4 as m4
+
+        T, K = 8192, 14336
+        x = torch.randn(T, K, device=dev).bfloat16()
+        q, s = m4.mx4_quantize_act(x)
+        for name, fn, per in (("act", lambda: m4.mx4_quantize_act(x), 2.53), ("weight", lambda: m4.mx4_quantize_weight_operands(x), 2.56),
+                              ("to_bf16", lambda: m4.mx4_dequantize(q, s), 2.53), ("to_e4m3", lambda: m4.mx4_to_e4m3(q), 1.5)):
+            ms = _time(fn, args.iters)
+            out.update({f"{name}_ms": ms, f"{name}_gbs": T * K * per / ms / 1e6})
+    elif args.case == "token_logprobs":
+        from flex_shard_b200.ops.logprobs import token_logprobs
+
+        T, V = 4096, 128256
+        x = (torch.randn(T, V, device=dev) * 2).bfloat16()
+        t = torch.randint(0, V, (T,), device=dev)
+        with torch.no_grad():
+            for k in (0, 8):
+                ms = _time(lambda: token_logprobs(x, t, top_k=k), args.iters)
+                out.update({f"forward_top{k}_ms": ms, f"forward_top{k}_gbs": T * V * 2 / ms / 1e6})
+        x.requires_grad_()
+        res = token_logprobs(x, t)
+        g = [torch.randn_like(res.logprob), torch.randn_like(res.entropy)]
+        ms = _time(lambda: torch.autograd.grad([res.logprob, res.entropy], x, g, retain_graph=True), args.iters)
+        out.update(T=T, V=V, gradient_ms=ms, gradient_gbs=T * V * 4 / ms / 1e6)
     elif args.case == "allgather_gemm":
         # 8 emulated peers on one GPU (the stager CTAs run the same bulk-copy ring; on a multi-GPU
         # job the sources are NVLink peer addresses instead of local ones)
