@@ -58,10 +58,15 @@ template <typename T> struct Vec;     // 16 bytes: L elements
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int L = 8;
   static constexpr uint32_t NEG_INF = 0xff80ff80u;
-  static __device__ __forceinline__ float largest(const uint4& v) {   // a NaN if there is one
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-    const float2 m = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
-    return max_nan(m.x, m.y);
+  static __device__ __forceinline__ float largest(const uint4 (&v)[4]) {   // a NaN if there is one
+    __nv_bfloat162 m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v[q]);
+      m[q] = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    }
+    const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3])));
+    return max_nan(f.x, f.y);
   }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -78,10 +83,15 @@ template <> struct Vec<__nv_bfloat16> {
 template <> struct Vec<__half> {
   static constexpr int L = 8;
   static constexpr uint32_t NEG_INF = 0xfc00fc00u;
-  static __device__ __forceinline__ float largest(const uint4& v) {
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
-    const float2 m = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
-    return max_nan(m.x, m.y);
+  static __device__ __forceinline__ float largest(const uint4 (&v)[4]) {
+    __half2 m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const __half2* h = reinterpret_cast<const __half2*>(&v[q]);
+      m[q] = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    }
+    const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3])));
+    return max_nan(f.x, f.y);
   }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
@@ -103,8 +113,12 @@ template <> struct Vec<__half> {
 template <> struct Vec<float> {
   static constexpr int L = 4;
   static constexpr uint32_t NEG_INF = 0xff800000u;
-  static __device__ __forceinline__ float largest(const uint4& v) {
-    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  static __device__ __forceinline__ float largest(const uint4 (&v)[4]) {
+    float m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      m[q] = max_nan(max_nan(__uint_as_float(v[q].x), __uint_as_float(v[q].y)), max_nan(__uint_as_float(v[q].z), __uint_as_float(v[q].w)));
+    return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
   }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
@@ -161,7 +175,7 @@ struct SumsSmem {
 };
 template <int THREADS>
 struct TopSmem {
-  unsigned long long lists[MAX_PARTS * 32];       // sorted alternatives of the row's parts (in the first CTA; 0: none)
+  unsigned long long lists[MAX_PARTS * MAX_TOP];  // alternatives of the row's parts (in the first CTA; 0: none)
   unsigned long long best[32];                    // ... of this part, then of the row
   unsigned long long cand[CAP];
   alignas(16) uint32_t groups[GROUPS];
@@ -308,9 +322,11 @@ __device__ __forceinline__ void part_top(const T* r, int first_vec, int end_vec,
 
 // One read of the logits: a row, or a part of it where there are few rows (the CTAs of a cluster then leave their sums and
 // alternatives with the first one). Every thread keeps a running maximum and sums relative to it, and the maxima of its chunks
-// for the alternatives.
+// for the alternatives. Bound by memory, closely followed by the issue of instructions (some ten an element at first): the
+// maximum of four vectors at a time and loads without bounds checks but for the row's rest, 8192 x 128256 bf16 343 -> 317 us
+// (6.6 TB/s) without alternatives, 432 -> 389 with 8.
 template <typename T, bool TOP, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1280 / THREADS)
+__global__ void __launch_bounds__(THREADS, (sizeof(T) == 4 ? 1536 : 1280) / THREADS)
 logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
                 long long ignore_index, int parts, float* __restrict__ logprob, float* __restrict__ entropy,
                 float2* __restrict__ stats, float* __restrict__ top_lp, long long* __restrict__ top) {
@@ -349,30 +365,24 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   const int cl_bits = max(2, 32 - __clz((n + MAX_CHUNKS - 1) / MAX_CHUNKS - 1));   // a chunk: 2^cl_bits vectors, 4 or more
   Sums a{floor_, 0.f, 0.f};
   float tmax = -INFINITY, cmax = -INFINITY;
-  auto take = [&](const uint4& v) {
-    float f[L];
-    Vec<T>::unpack(v, f);
+  int chunk = 0, in_chunk = 0;
+  auto take = [&](const uint4 (&v)[4]) {
     const float vm = Vec<T>::largest(v);
-    if (TOP) cmax = max_nan(cmax, vm);
     if (vm > a.m) a.raise(vm, c);
     const float mo = -a.m * c;
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      const float d = max_nan(fmaf(f[j], c, mo), -256.f), e = ex2(d);   // 2^-256 is 0: nothing from masked tokens
-      a.s += e;
-      a.u = fmaf(d, e, a.u);
+    for (int q = 0; q < 4; ++q) {
+      float f[L];
+      Vec<T>::unpack(v[q], f);
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const float d = max_nan(fmaf(f[j], c, mo), -256.f), e = ex2(d);   // 2^-256 is 0: nothing from masked tokens
+        a.s += e;
+        a.u = fmaf(d, e, a.u);
+      }
     }
-  };
-  const uint4* g = reinterpret_cast<const uint4*>(r + span.head);
-  const uint4 none = make_uint4(Vec<T>::NEG_INF, Vec<T>::NEG_INF, Vec<T>::NEG_INF, Vec<T>::NEG_INF);
-  int chunk = 0, in_chunk = 0;
-  for (int i = first_vec + tid; i < end_vec; i += 4 * THREADS) {
-    uint4 v[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = i + q * THREADS < end_vec ? load_stream(g + i + q * THREADS) : none;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) take(v[q]);
     if constexpr (TOP) {
+      cmax = max_nan(cmax, vm);
       in_chunk += 4;
       if (in_chunk == 1 << cl_bits) {
         ts.cmax[chunk++][tid] = cmax;
@@ -381,6 +391,22 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
         in_chunk = 0;
       }
     }
+  };
+  const uint4* g = reinterpret_cast<const uint4*>(r + span.head) + tid;
+  int i = first_vec;
+  for (; i + 4 * THREADS <= end_vec; i += 4 * THREADS) {
+    uint4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = load_stream(g + i + q * THREADS);
+    take(v);
+  }
+  if (i + tid < end_vec) {                            // the rest of the row; absent vectors hold minus infinity
+    uint4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      v[q] = i + q * THREADS + tid < end_vec ? load_stream(g + i + q * THREADS)
+                                             : make_uint4(Vec<T>::NEG_INF, Vec<T>::NEG_INF, Vec<T>::NEG_INF, Vec<T>::NEG_INF);
+    take(v);
   }
   if constexpr (TOP) {
     tmax = max_nan(tmax, cmax);
@@ -446,8 +472,10 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(all.s) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(all.u) : "memory");
       }
-      if constexpr (TOP)
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_cta(smem_u32(&ts.lists[part * 32 + lane]), 0)), "l"(ts.best[lane]) : "memory");
+      if constexpr (TOP) {
+        if (lane < k)
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_cta(smem_u32(&ts.lists[part * k + lane]), 0)), "l"(ts.best[lane]) : "memory");
+      }
     }
     __syncwarp();
     cluster_sync_all();
@@ -456,7 +484,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     if constexpr (TOP) {
       if (tid < 32) ts.best[tid] = 0;
       __syncthreads();
-      rank_keys<THREADS>(ts.lists, parts * 32, ts.best);
+      rank_keys<THREADS>(ts.lists, parts * k, ts.best);
       __syncthreads();
     }
   }
@@ -589,15 +617,16 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ targe
 
 constexpr int SMALL = 128, LARGE = 256;     // threads of a CTA
 
-// CTAs of a row: as many as `places` allow, with 4096 elements or more each.
-int row_parts(long long T, int V, int places) {
+// CTAs of a row: as many as `places` allow (two already where `first` does), with 4096 elements or more each.
+int row_parts(long long T, int V, int first, int places) {
   int parts = 1;
-  while (parts < MAX_PARTS && T * parts * 2 <= places && V / (parts * 2) >= 4096) parts *= 2;
+  while (parts < MAX_PARTS && T * parts * 2 <= (parts == 1 ? first : places) && V / (parts * 2) >= 4096) parts *= 2;
   return parts;
 }
 // Small CTAs, of which an SM holds ten, hide the ends of short rows; a long row, or the only one an SM has, streams faster into a
 // large one. Forward with 8 alternatives, 128 / 256 threads: 20000 x 2000 bf16 95 / 174 us, 6000 x 12000 47 / 72, 8192 x 32000
-// 122 / 143, 4096 x 64000 104 / 113, 4096 x 128256 199 / 199, 1500 x 50021 fp32 63 / 59, 148 x 128256 30 / 19.
+// 122 / 143, 4096 x 64000 104 / 113, 4096 x 128256 199 / 199, 1500 x 50021 fp32 63 / 59, 148 x 128256 30 / 19. CTAs of 512 threads,
+// two to an SM: 8192 x 128256 466 / 389.
 bool small_ctas(long long ctas, int V, int size) { return V <= 8192 || (static_cast<long long>(V) * size <= 128 * 1024 && ctas >= 592); }
 
 inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH; }
@@ -611,9 +640,10 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
   if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2) return FSB_ERR_BAD_ARG;
   if (T > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   if (T == 0) return FSB_OK;
-  // One CTA an SM is enough: with alternatives the parts' exchange costs more than it gains (74 x 128256, 2 / 4 / 8 parts: 10.3,
-  // 12.7, 19.8 us; 7 rows 8 parts 9.1), without it is even (7.3, 8.1, 8.3).
-  const int parts = row_parts(T, V, 148);
+  // Two CTAs of 256 threads for an SM's only row (148 x 128256: 10.1 / 13.4 us without and with 8 alternatives, one CTA 16.1 /
+  // 18.5); more parts only towards one an SM, since their exchange costs more than it gains (74 x 128256 with alternatives, 2 / 4
+  // / 8 parts: 10.3, 12.7, 19.8 us; without 7.3, 8.1, 8.3).
+  const int parts = row_parts(T, V, 296, 148);
   if (T * parts > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(T * parts), 1, 1);
@@ -653,7 +683,7 @@ FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* tar
   // 108 us; 1000 x 50000 bf16, 1 / 4: 45 / 38), not more (4096 x 128256, 1 / 8: 339 / 368).
   auto run = [&](auto* p) {
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    const dim3 grid(static_cast<unsigned>(T), row_parts(T, V, 4096));
+    const dim3 grid(static_cast<unsigned>(T), row_parts(T, V, 4096, 4096));
     const bool small = V <= 8192;     // longer rows: even (8192 x 32000 187 / 189 us, 4096 x 128256 362 / 350)
     auto kernel = small ? logprobs_bwd_kernel<E, SMALL> : logprobs_bwd_kernel<E, LARGE>;
     kernel<<<grid, small ? SMALL : LARGE, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
