@@ -309,38 +309,45 @@ __device__ __forceinline__ void store4(const Args& args, int t, int n, const flo
       if (n + i < args.N) d[i] = __float2bfloat16(f[i]);
   }
 }
-// Epilogue of the one-SM kernels: the 128 threads of the epilogue warps have left their CTA's sums [rows][128] at `smem` (a
+// End of the one-SM kernels, for all threads of a CTA: its epilogue warps (2 to 5) have left its sums [rows][128] at `smem` (a
 // thread there has one weight row, 2 bytes of each output row; here it stores 8 of one). With several CTAs along K the cluster's
 // sums are added in CTA order and the CTAs divide the rows; all parts' 16 bytes are on their way before the first is added.
-__device__ __forceinline__ void store_rows(const Args& args, const uint8_t* smem, int part, int t0, int rows, int n0, int thread) {
-  const int n = thread % 32 * 4;
+__device__ __forceinline__ void store_rows(const Args& args, const uint8_t* smem, int part, int t0, int rows, int n0) {
+  const int thread = static_cast<int>(threadIdx.x) - 64, n = thread % 32 * 4;
   if (args.split == 1) {
+    if (thread < 0) return;
     asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll 4
     for (int t = thread / 32; t < rows; t += 4) store4(args, t0 + t, n0 + n, *reinterpret_cast<const float4*>(smem + (t * BM + n) * 4));
     return;
   }
-  const int per = (rows + args.split - 1) / args.split, end = min((part + 1) * per, rows);
+  __syncwarp();
+  cluster_sync_all();
+  if (thread >= 0) {
+    const int per = (rows + args.split - 1) / args.split, end = min((part + 1) * per, rows);
 #pragma unroll 2
-  for (int t = part * per + thread / 32; t < end; t += 4) {
-    const uint32_t own = smem_u32(smem) + (t * BM + n) * 4;
-    float4 o[MAX_SPLIT], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int t = part * per + thread / 32; t < end; t += 4) {
+      const uint32_t own = smem_u32(smem) + (t * BM + n) * 4;
+      float4 o[MAX_SPLIT], sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int p = 0; p < MAX_SPLIT; ++p) {
-      o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p < args.split)
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(o[p].x), "=f"(o[p].y), "=f"(o[p].z), "=f"(o[p].w) : "r"(map_to_cta(own, p)));
-    }
+      for (int p = 0; p < MAX_SPLIT; ++p) {
+        o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < args.split)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(o[p].x), "=f"(o[p].y), "=f"(o[p].z), "=f"(o[p].w) : "r"(map_to_cta(own, p)));
+      }
 #pragma unroll
-    for (int p = 0; p < MAX_SPLIT; ++p) {
-      sum.x += o[p].x;
-      sum.y += o[p].y;
-      sum.z += o[p].z;
-      sum.w += o[p].w;
+      for (int p = 0; p < MAX_SPLIT; ++p) {
+        sum.x += o[p].x;
+        sum.y += o[p].y;
+        sum.z += o[p].z;
+        sum.w += o[p].w;
+      }
+      store4(args, t0 + t, n0 + n, sum);
     }
-    store4(args, t0 + t, n0 + n, sum);
   }
+  __syncwarp();
+  cluster_sync_all();                                          // the others' sums have been read
 }
 
 template <int BN>
@@ -472,15 +479,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
     tc_fence_before();
   }
-  if (args.split > 1) {
-    __syncwarp();
-    cluster_sync_all();
-  }
-  if (warp >= 2) store_rows(args, smem, part, tx * BN, rows, tw * BM, static_cast<int>(threadIdx.x) - 64);
-  if (args.split > 1) {
-    __syncwarp();
-    cluster_sync_all();                                        // the others' sums have been read
-  }
+  store_rows(args, smem, part, tx * BN, rows, tw * BM);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -648,15 +647,7 @@ linear_mxfp4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 #pragma unroll
     for (int i = 0; i < F_BN; ++i) reinterpret_cast<float*>(smem)[i * BM + n_local] = acc[i];   // the first stage is free by now
   }
-  if (args.split > 1) {
-    __syncwarp();
-    cluster_sync_all();
-  }
-  if (warp >= 2) store_rows(args, smem, part, 0, args.M, tw * BM, static_cast<int>(threadIdx.x) - 64);
-  if (args.split > 1) {
-    __syncwarp();
-    cluster_sync_all();                                       // the others' sums have been read
-  }
+  store_rows(args, smem, part, 0, args.M, tw * BM);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
