@@ -37,7 +37,8 @@ def gradient(x, target, temperature, k, g, h, gt, ignore_index=-100):
     if k:
         dz.scatter_add_(1, torch.where(live[:, None], out["top_index"], 0), gt)
     size = p * (g.abs() + gt.abs().sum(1))[:, None] + p * h.abs()[:, None] * (flat.abs() + H + 1)
-    return dz / temperature, size / temperature
+    dead = ~live[:, None]                   # ignored rows are not read, whatever they hold
+    return dz.masked_fill(dead, 0.0) / temperature, size.masked_fill(dead, 0.0) / temperature
 
 
 def value_tolerance(x, temperature):
@@ -50,5 +51,9 @@ def value_tolerance(x, temperature):
     return (2 * top + 16 + math.log(V)) * 2.0 ** -22 + (V / 256 + 16) * 2.0 ** -24
 
 
-HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -23}   # fp32: the last two operations
+# Relative error of a gradient besides what `gradient`'s second result scales. At a position that is the target and an
+# alternative the kernel computes fl(fl(a) fl(1 / temperature) + ...) with a = fl(g + g_i): four fp32 roundings of 2^-24 each
+# (sum, reciprocal, product, last sum), 2^-22 together; 16-bit gradients are rounded once more, by half a step.
+FP32_STEPS = 2.0 ** -22
+HALF_STEP = {torch.bfloat16: 2.0 ** -8 + FP32_STEPS, torch.float16: 2.0 ** -11 + FP32_STEPS, torch.float32: FP32_STEPS}
 SMALLEST = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -126}
