@@ -141,7 +141,10 @@ def device_of(tensor):
 def plain(*tensors) -> bool:
     """Whether a kernel may be given these tensors' addresses: no subclasses, and no tensors without memory of their own
     (those that ``vmap``, batched gradients and the ``torch.func`` transforms hand to an operator)."""
-    return all(type(t) in (torch.Tensor, torch.nn.Parameter) and torch._C._has_storage(t) for t in tensors)
+    for t in tensors:
+        if type(t) not in (torch.Tensor, torch.nn.Parameter) or not torch._C._has_storage(t):
+            return False
+    return True
 
 
 STATUS_INTS = 8     # [0] code; a failed peer wait also leaves [1],[2] flag address, [3] epoch, [4] peer, [5] value seen

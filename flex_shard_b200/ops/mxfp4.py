@@ -53,11 +53,12 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
 
 
 def _check_operand(q: torch.Tensor, scales: torch.Tensor, what: str) -> None:
-    if q.dim() != 2 or q.dtype != torch.uint8 or q.shape[1] % (GROUP // 2) or q.shape[1] == 0:
+    shape = q.shape
+    if len(shape) != 2 or q.dtype is not torch.uint8 or shape[1] % (GROUP // 2) or shape[1] == 0:
         raise ValueError(f"{what}: codes must be a uint8 matrix [rows, cols / 2] with cols a multiple of {GROUP}, got "
-                         f"{q.dtype}{tuple(q.shape)}")
-    need = blocked_scale_numel(q.shape[0], 2 * q.shape[1])
-    if scales.dtype != torch.uint8 or scales.numel() < need or not scales.is_contiguous() or scales.device != q.device:
+                         f"{q.dtype}{tuple(shape)}")
+    need = (-(-shape[0] // 128) * 128) * (-(-shape[1] // 64) * 4)        # blocked_scale_numel(rows, cols)
+    if scales.dtype is not torch.uint8 or scales.numel() < need or not scales.is_contiguous() or scales.device != q.device:
         raise ValueError(f"{what}: scales must be at least {need} contiguous uint8 bytes in block layout on the codes' device")
 
 
