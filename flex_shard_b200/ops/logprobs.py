@@ -2,8 +2,8 @@
 (``csrc/logprobs.cu``). The counterpart of ``cross_entropy`` where a value per token is wanted: policy gradients,
 distillation on a teacher's alternatives, scoring.
 
-CPU tensors take a PyTorch restatement of the same arithmetic, and so do ``torch.func`` transforms, forward-mode derivatives and
-batched gradients.
+CPU tensors take a PyTorch restatement of the same arithmetic, and so do ``torch.func`` transforms, forward-mode derivatives,
+batched gradients and gradients that are differentiated again.
 """
 from __future__ import annotations
 
@@ -52,7 +52,7 @@ def _restatement(x, target, temperature, k, ignore_index):
     V = x.shape[1]
     live = target != ignore_index
     valid = live & (target >= 0) & (target < V)
-    xf = x.float()
+    xf = torch.where(live[:, None], x, 0).float()       # ignored rows take no part, whatever they hold
     lp = torch.log_softmax((xf - xf.detach().amax(-1, keepdim=True)) / temperature, -1)
     at = torch.where(valid, target, 0)
     # a target outside the vocabulary makes its row's value and gradient NaN
@@ -127,7 +127,6 @@ class _TokenLogprobs(torch.autograd.Function):
         return logprob, entropy, top_lp, top
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, glp, gh, gtop, _):
         x, target, top, stats, entropy = ctx.saved_tensors
         temperature, ignore_index = ctx.cfg
@@ -138,6 +137,10 @@ class _TokenLogprobs(torch.autograd.Function):
         given = [g for g in (glp, gh, gtop) if g is not None]
         if not given:
             return None, None, None, None, None
+        if torch.is_grad_enabled():     # a gradient that may be differentiated again: PyTorch's own derivatives
+            outs = _restatement(x, target, temperature, k, ignore_index)
+            (dx,) = torch.autograd.grad([o for o, g in zip(outs, (glp, gh, gtop)) if g is not None], x, given, create_graph=True)
+            return dx, None, None, None, None
         if not x.is_cuda or not _lib.plain(*given):
             return _restated_gradient(x, target, top, stats, entropy, temperature, ignore_index, glp, gh, gtop), None, None, None, None
         glp, gh, gtop = (None if g is None else g.float().contiguous() for g in (glp, gh, gtop))

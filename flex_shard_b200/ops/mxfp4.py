@@ -285,6 +285,7 @@ class _Mxfp4Linear(torch.autograd.Function):
         return _product_with(x2, wq, fwd_scale).view(*x.shape[:-1], wq.shape[0])
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x2, wq, dgrad_scale = ctx.saved_tensors
         weight = ctx.weight

@@ -151,9 +151,13 @@ def test_parts_of_the_gradient():
     g[2] = 0
     (dy,) = torch.autograd.grad(token_logprobs(y, t).logprob, y, g)
     assert not dy[2].any() and dy[[0, 1, 3, 4]].any(1).all()
-    with pytest.raises(RuntimeError):
-        (d,) = torch.autograd.grad(token_logprobs(x, t).logprob.sum(), x, create_graph=True)
-        d.sum().backward()
+    # a gradient that can be differentiated again is the same gradient
+    for which in range(3):
+        g = torch.randn_like(token_logprobs(x, t, top_k=4)[which])
+        (a,) = torch.autograd.grad(token_logprobs(x, t, top_k=4)[which], x, g)
+        (b,) = torch.autograd.grad(token_logprobs(x, t, top_k=4)[which], x, g, create_graph=True)
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
+        assert torch.autograd.grad(b.square().sum(), x)[0].isfinite().all()
 
 
 def test_batched_gradients():

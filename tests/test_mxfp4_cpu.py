@@ -148,6 +148,14 @@ def test_no_rows():
     assert y.shape == (0, 128) and dx.shape == (0, 128) and not dw.any()
 
 
+def test_second_derivatives_are_refused():
+    x, w = torch.randn(4, 128).bfloat16().requires_grad_(), torch.randn(128, 128).bfloat16()
+    w4 = BlockwiseMxfp4Weight.from_float(w)
+    (dx,) = torch.autograd.grad(m4.mxfp4_linear(x, None, w4.qdata, w4.scale, w4.dgrad_scale).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.float().sum().backward()
+
+
 def test_refusals():
     x, w = torch.zeros(4, 128).bfloat16(), torch.zeros(128, 128).bfloat16()
     w4 = BlockwiseMxfp4Weight.from_float(w)
