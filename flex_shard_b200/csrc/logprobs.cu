@@ -128,6 +128,14 @@ template <> struct Vec<float> {
   }
 };
 
+// Rows of a tensor [batches, inner, V]: batches `ldb` elements apart, their rows `ld`.
+struct Rows {
+  long long inner, ldb, ld;
+  template <typename T>
+  __device__ __forceinline__ const T* at(const T* x, long long row) const {
+    return inner == 0 ? x + row * ld : x + row / inner * ldb + row % inner * ld;
+  }
+};
 // A row as whole 16-byte vectors between a head and a tail of single elements.
 struct RowSpan {
   int head, nvec, tail;
@@ -327,7 +335,7 @@ __device__ __forceinline__ void part_top(const T* r, int first_vec, int end_vec,
 // (6.6 TB/s) without alternatives, 432 -> 389 with 8.
 template <typename T, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, (sizeof(T) == 4 ? 1536 : 1280) / THREADS)
-logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
+logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, const Rows rows, float inv_t, int k,
                 long long ignore_index, int parts, float* __restrict__ logprob, float* __restrict__ entropy,
                 float2* __restrict__ stats, float* __restrict__ top_lp, long long* __restrict__ top) {
   constexpr int L = Vec<T>::L, WARPS = THREADS / 32;
@@ -335,7 +343,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   __shared__ typename std::conditional<TOP, TopSmem<THREADS>, int>::type ts;
   const long long row = blockIdx.x / parts;
   const int part = static_cast<int>(blockIdx.x % parts);
-  const T* r = x + row * ld;
+  const T* r = rows.at(x, row);
   const long long tgt = target[row];
   const int tid = threadIdx.x, lane = tid & 31;
   if (tgt == ignore_index) {                         // the same for every CTA of the row: none of them meets a barrier
@@ -528,13 +536,13 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
 // Row blockIdx.x, part blockIdx.y. With l = log2 p_j the first term is p_j (l A + B); the chosen positions are written again.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1280 / THREADS)
-logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, long long ld, float inv_t, int k,
+logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, const Rows rows, float inv_t, int k,
                     long long ignore_index, const long long* __restrict__ top, const float2* __restrict__ stats,
                     const float* __restrict__ entropy, const float* __restrict__ glp, const float* __restrict__ gh,
                     const float* __restrict__ gtop, T* __restrict__ dx, long long ldd) {
   constexpr int L = Vec<T>::L;
   const long long row = blockIdx.x;
-  const T* r = x + row * ld;
+  const T* r = rows.at(x, row);
   T* d = dx + row * ldd;
   const long long tgt = target[row];
   const int tid = threadIdx.x;
@@ -632,12 +640,14 @@ bool small_ctas(long long ctas, int V, int size) { return V <= 8192 || (static_c
 inline int ok() { return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH; }
 }  // namespace
 
-// kind: 0 bf16, 1 fp16, 2 fp32. x [T, V] with row stride ld elements; logprob, entropy [T]; stats [T, 2] (maximum
+// kind: 0 bf16, 1 fp16, 2 fp32. x: T rows of V elements, ld elements apart; with inner > 0 in batches of `inner` rows that start ldb
+// elements apart. logprob, entropy [T]; stats [T, 2] (maximum
 // and log s, for the backward pass; may be null); top_lp, top [T, k].
-FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target, long long T, int V, long long ld, float inv_t,
-                               int k, long long ignore_index, float* logprob, float* entropy, void* stats, float* top_lp,
+FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target, long long T, int V, long long inner, long long ldb,
+                               long long ld, float inv_t, int k, long long ignore_index, float* logprob, float* entropy, void* stats, float* top_lp,
                                long long* top, cudaStream_t stream) {
-  if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2) return FSB_ERR_BAD_ARG;
+  if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2 || inner < 0) return FSB_ERR_BAD_ARG;
+  const Rows rows{inner, ldb, ld};
   if (T > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   if (T == 0) return FSB_OK;
   // Two CTAs of 256 threads for an SM's only row (148 x 128256: 10.1 / 13.4 us without and with 8 alternatives, one CTA 16.1 /
@@ -661,7 +671,7 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
     using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
     auto kernel = k > 0 ? (small ? logprobs_kernel<E, true, SMALL> : logprobs_kernel<E, true, LARGE>)
                         : (small ? logprobs_kernel<E, false, SMALL> : logprobs_kernel<E, false, LARGE>);
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p, target, V, ld, inv_t, k, ignore_index, parts, logprob, entropy,
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p, target, V, rows, inv_t, k, ignore_index, parts, logprob, entropy,
                                                static_cast<float2*>(stats), top_lp, top);
     const int rc = ok();   // also clears the error of a launch that failed
     return err == cudaSuccess ? rc : static_cast<int>(FSB_ERR_LAUNCH);
@@ -672,11 +682,12 @@ FSB_API int fsb_token_logprobs(const void* x, int kind, const long long* target,
 }
 
 // top, stats, entropy as the forward left them; glp, gh [T], gtop [T, k] (each may be null); dx [T, V] with row stride ldd.
-FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* target, long long T, int V, long long ld, float inv_t,
-                                   int k, long long ignore_index, const long long* top, const void* stats, const float* entropy,
+FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* target, long long T, int V, long long inner,
+                                   long long ldb, long long ld, float inv_t, int k, long long ignore_index, const long long* top, const void* stats, const float* entropy,
                                    const float* glp, const float* gh, const float* gtop, void* dx, long long ldd,
                                    cudaStream_t stream) {
-  if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2) return FSB_ERR_BAD_ARG;
+  if (T < 0 || V <= 0 || k < 0 || k > MAX_TOP || k > V || kind < 0 || kind > 2 || inner < 0) return FSB_ERR_BAD_ARG;
+  const Rows rows{inner, ldb, ld};
   if (T > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
   if (T == 0) return FSB_OK;
   // Parts have nothing to exchange here: up to 4096 CTAs, so that the last wave weighs little (1500 x 50021 fp32, 1 / 2 parts: 116 /
@@ -686,7 +697,7 @@ FSB_API int fsb_token_logprobs_bwd(const void* x, int kind, const long long* tar
     const dim3 grid(static_cast<unsigned>(T), row_parts(T, V, 4096, 4096));
     const bool small = V <= 8192;     // longer rows: even (8192 x 32000 187 / 189 us, 4096 x 128256 362 / 350)
     auto kernel = small ? logprobs_bwd_kernel<E, SMALL> : logprobs_bwd_kernel<E, LARGE>;
-    kernel<<<grid, small ? SMALL : LARGE, 0, stream>>>(p, target, V, ld, inv_t, k, ignore_index, top,
+    kernel<<<grid, small ? SMALL : LARGE, 0, stream>>>(p, target, V, rows, inv_t, k, ignore_index, top,
                                                        static_cast<const float2*>(stats), entropy, glp, gh, gtop,
                                                        static_cast<E*>(dx), ldd);
     return ok();

@@ -36,8 +36,8 @@ def _ensure():
     if not _declared:
         c = ctypes
         vp, i32, i64, f32 = c.c_void_p, c.c_int, c.c_longlong, c.c_float
-        _lib.declare("fsb_token_logprobs", [vp, i32, vp, i64, i32, i64, f32, i32, i64, vp, vp, vp, vp, vp, vp])
-        _lib.declare("fsb_token_logprobs_bwd", [vp, i32, vp, i64, i32, i64, f32, i32, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp])
+        _lib.declare("fsb_token_logprobs", [vp, i32, vp, i64, i32, i64, i64, i64, f32, i32, i64, vp, vp, vp, vp, vp, vp])
+        _lib.declare("fsb_token_logprobs_bwd", [vp, i32, vp, i64, i32, i64, i64, i64, f32, i32, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp])
         _declared = True
 
 
@@ -48,8 +48,9 @@ def _top_indices(x: torch.Tensor, k: int) -> torch.Tensor:
 
 
 def _restatement(x, target, temperature, k, ignore_index):
-    """The operator in differentiable PyTorch operations, on ``[T, V]`` logits."""
-    V = x.shape[1]
+    """The operator in differentiable PyTorch operations."""
+    V = x.shape[-1]
+    x = x.reshape(-1, V)
     live = target != ignore_index
     valid = live & (target >= 0) & (target < V)
     xf = torch.where(live[:, None], x, 0).float()       # ignored rows take no part, whatever they hold
@@ -68,7 +69,8 @@ def _restatement(x, target, temperature, k, ignore_index):
 
 def _restated_gradient(x, target, top, stats, entropy, temperature, ignore_index, glp, gh, gtop):
     """The gradient's formula in PyTorch operations (gradients may be batched)."""
-    V = x.shape[1]
+    shape, V = x.shape, x.shape[-1]
+    x = x.reshape(-1, V)
     live = target != ignore_index
     valid = live & (target >= 0) & (target < V)
     lp = (x.float() - stats[:, :1]) / temperature - stats[:, 1:]
@@ -87,17 +89,23 @@ def _restated_gradient(x, target, top, stats, entropy, temperature, ignore_index
         for i in range(top.shape[1]):
             dz = dz + gtop[:, i, None] * ((cols == top[:, i, None]).float() - p)
             wanted = wanted | (gtop[:, i] != 0)
-    return (torch.where((live & wanted)[:, None], dz, 0.0) / temperature).to(x.dtype)
+    return (torch.where((live & wanted)[:, None], dz, 0.0) / temperature).to(x.dtype).reshape(shape)
+
+
+def _rows(x):
+    """How the kernels find the rows of ``[T, V]`` or ``[batches, rows, V]`` logits."""
+    return (0, 0, x.stride(0)) if x.dim() == 2 else (x.shape[1], x.stride(0), x.stride(1))
 
 
 def _forward(x, target, temperature, k, ignore_index, stats):
-    """``stats`` [T, 2] takes the numbers of a row that the gradient starts from, the largest logit and the logarithm of the
+    """``x`` is ``[T, V]`` or ``[batches, rows, V]`` with ``T`` rows in all. ``stats`` [T, 2] takes the numbers of a row that the gradient starts from, the largest logit and the logarithm of the
     sum relative to it (``None``: not wanted)."""
-    T, V = x.shape
+    T, V = target.shape[0], x.shape[-1]
     if not x.is_cuda:
         if stats is not None:
-            m = x.float().amax(-1, keepdim=True)
-            stats.copy_(torch.cat([m, ((x.float() - m) / temperature).exp().sum(-1, keepdim=True).log()], -1))
+            xf = x.reshape(-1, V).float()
+            m = xf.amax(-1, keepdim=True)
+            stats.copy_(torch.cat([m, ((xf - m) / temperature).exp().sum(-1, keepdim=True).log()], -1))
         return _restatement(x, target, temperature, k, ignore_index)
     _ensure()
     dev = x.device
@@ -106,7 +114,7 @@ def _forward(x, target, temperature, k, ignore_index, stats):
     top_lp = torch.empty(T, k, dtype=torch.float32, device=dev)
     top = torch.empty(T, k, dtype=torch.int64, device=dev)
     with _lib.device_of(x):
-        rc = _lib.load().fsb_token_logprobs(x.data_ptr(), _KINDS[x.dtype], target.data_ptr(), T, V, x.stride(0), 1.0 / temperature,
+        rc = _lib.load().fsb_token_logprobs(x.data_ptr(), _KINDS[x.dtype], target.data_ptr(), T, V, *_rows(x), 1.0 / temperature,
                                             k, ignore_index, logprob.data_ptr(), entropy.data_ptr(),
                                             None if stats is None else stats.data_ptr(), top_lp.data_ptr(), top.data_ptr(),
                                             _lib.stream_ptr(dev))
@@ -118,7 +126,7 @@ def _forward(x, target, temperature, k, ignore_index, stats):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, target, temperature, k, ignore_index):
-        stats = torch.empty(x.shape[0], 2, dtype=torch.float32, device=x.device)
+        stats = torch.empty(target.shape[0], 2, dtype=torch.float32, device=x.device)
         logprob, entropy, top_lp, top = _forward(x, target, temperature, k, ignore_index, stats)
         ctx.save_for_backward(x, target, top, stats, entropy)
         ctx.cfg = (temperature, ignore_index)
@@ -130,7 +138,7 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, glp, gh, gtop, _):
         x, target, top, stats, entropy = ctx.saved_tensors
         temperature, ignore_index = ctx.cfg
-        T, V = x.shape
+        T, V = target.shape[0], x.shape[-1]
         k = top.shape[1]
         if k == 0:
             gtop = None
@@ -146,11 +154,11 @@ class _TokenLogprobs(torch.autograd.Function):
         glp, gh, gtop = (None if g is None else g.float().contiguous() for g in (glp, gh, gtop))
         # rows of the gradient start as far into 16 bytes as the logits' rows do, so that both move in whole vectors
         lanes = 16 // x.element_size()
-        ld = V + (x.stride(0) - V) % lanes if T > 1 else V
-        dx = torch.empty(T * ld, dtype=x.dtype, device=x.device).view(T, ld)[:, :V]
+        ld = V + (x.stride(-2) - V) % lanes if T > 1 else V
+        dx = torch.empty(*x.shape[:-1], ld, dtype=x.dtype, device=x.device)[..., :V]
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         with _lib.device_of(x):
-            rc = _lib.load().fsb_token_logprobs_bwd(x.data_ptr(), _KINDS[x.dtype], target.data_ptr(), T, V, x.stride(0),
+            rc = _lib.load().fsb_token_logprobs_bwd(x.data_ptr(), _KINDS[x.dtype], target.data_ptr(), T, V, *_rows(x),
                                                     1.0 / temperature, k, ignore_index, top.data_ptr(), stats.data_ptr(),
                                                     entropy.data_ptr(), ptr(glp), ptr(gh), ptr(gtop), dx.data_ptr(), ld,
                                                     _lib.stream_ptr(x.device))
@@ -163,7 +171,8 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, *, temperature: f
                    ignore_index: int = -100) -> TokenLogprobs:
     """``log softmax(logits / temperature)`` at ``target``, the distribution's entropy and its ``top_k`` likeliest tokens.
 
-    ``logits [..., V]`` bf16, fp16 or fp32 (rows may be strided), ``target [...]`` integer; ``top_k`` up to 32 and V. All
+    ``logits [..., V]`` bf16, fp16 or fp32 (strided rows, and batches of rows such as ``logits[:, :-1]``, are read where they
+    lie), ``target [...]`` integer; ``top_k`` up to 32 and V. All
     arithmetic in fp32; the logits are read once and left as they are. Differentiable with respect to ``logits`` through
     ``logprob``, ``entropy`` and ``top_logprob`` (the choice of alternatives counts as constant); the backward pass reads the
     logits again, so they must not be overwritten before it (as ``cross_entropy`` does).
@@ -193,11 +202,14 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, *, temperature: f
     lead = target.shape
     x, t = logits, target
     if len(lead) != 1:
-        x, t = x.reshape(-1, V), t.reshape(-1)
+        t = t.reshape(-1)
+        # batches of rows (all positions but a sequence's last, for instance) are taken where they lie
+        if not (len(lead) == 2 and x.is_cuda and x.stride(2) == 1 and x.stride(0) != lead[1] * x.stride(1) and t.numel()):
+            x = x.reshape(-1, V)
     if t.dtype != torch.int64:
         t = t.long()
     if _lib.plain(logits, target) and forward_ad._current_level < 0:
-        if V > 1 and x.stride(1) != 1:
+        if V > 1 and x.stride(-1) != 1:
             x = x.contiguous()
         if not t.is_contiguous():
             t = t.contiguous()

@@ -226,3 +226,35 @@ def test_large_logits_that_few_threads_hold(V, period, held, dtype):
     x[2, where] += 30
     for k in (31, 32):
         check(x.to(dtype), torch.tensor([3, V - 1, 7], device="cuda"), 1.0, k)
+
+
+@pytest.mark.parametrize("B,S,V,dtype", [(3, 5, 1000, BF), (2, 9, 1001, BF), (4, 2, 33, FP), (2, 700, 4096, HF), (1, 6, 500, BF)])
+def test_batches_of_rows_where_they_lie(B, S, V, dtype):
+    """All positions but the last of every sequence, and every second one: the same numbers as from a copy, without one. Rows that
+    start elsewhere within 16 bytes than the copy's (an odd vocabulary) are added in another order: twice the sums' error."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    logits = (torch.randn(B, S + 1, V, generator=g, device="cuda") * 3).to(dtype)
+    t = torch.randint(0, V, (B, S), generator=g, device="cuda")
+    t[0, 0] = -100
+    for view in (logits[:, :-1], logits[:, 1:], logits.repeat(1, 2, 1)[:, ::2][:, :S], logits.transpose(0, 1)[:S].transpose(0, 1)):
+        x, y = view.detach().requires_grad_(), view.detach().clone(memory_format=torch.contiguous_format).requires_grad_()
+        a, b = token_logprobs(x, t, top_k=3), token_logprobs(y, t, top_k=3)
+        w = [torch.randn(o.shape, generator=g, device="cuda") for o in a[:3]]
+        (dx,), (dy,) = torch.autograd.grad(a[:3], x, w), torch.autograd.grad(b[:3], y, w)
+        assert dx.shape == view.shape and torch.equal(a.top_index, b.top_index)
+        if V * x.element_size() % 16 == 0:
+            assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(dx, dy)
+            continue
+        tol = 2 * value_tolerance(y.detach().view(-1, V), 1.0) * (1 + math.log(V))
+        for p, q in zip(a[:3], b[:3]):
+            torch.testing.assert_close(p, q, rtol=0, atol=tol)
+        want, size = gradient(y.detach().view(-1, V), t.view(-1), 1.0, 3, w[0].view(-1), w[1].view(-1), w[2].view(-1, 3))
+        for d in (dx, dy):
+            off = (d.double().reshape(-1, V) - want).abs()
+            assert (off <= want.abs() * HALF_STEP[dtype] + size * 8 * tol + SMALLEST[dtype]).all()
+    before = torch.cuda.max_memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    now = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        token_logprobs(logits[:, :-1], t)
+    assert torch.cuda.max_memory_allocated() - now < logits[:, :-1].numel() * logits.element_size() // 2 + 65536, before
