@@ -113,18 +113,22 @@ mx_quant_weight_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __restrict_
 
 // Tile exponents [ceil(rows/32), ceil(cols/32)] -> blocked scales for the operand [rows, cols]
 // (transpose == 0: groups run along the columns) or for its transpose [cols, rows] (groups run
-// along the rows). Padding rows / groups get exponent 127 (scale 1).
-__global__ void mx_expand_scales_kernel(const uint8_t* __restrict__ tile_exp, uint8_t* __restrict__ out, int op_rows,
-                                        int op_groups, int pad_rows, int pad_groups, int exp_cols, int transpose) {
-  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-  const long long total = static_cast<long long>(pad_rows) * pad_groups;
-  if (i >= total) return;
-  const long long r = i / pad_groups;
-  const int g = static_cast<int>(i % pad_groups);
-  uint8_t e = 127;
-  if (r < op_rows && g < op_groups)
-    e = transpose ? tile_exp[static_cast<long long>(g) * exp_cols + (r >> 5)] : tile_exp[(r >> 5) * exp_cols + g];
-  out[blocked_offset(r, g, pad_groups >> 2)] = e;
+// along the rows). Padding rows / groups get exponent 127 (scale 1). A CTA writes one 512-byte block,
+// a thread a word: row t / 4 of the 32-row slice t % 4, four groups.
+__global__ void __launch_bounds__(128)
+mx_expand_scales_kernel(const uint8_t* __restrict__ tile_exp, uint8_t* __restrict__ out, int op_rows, int op_groups, int n_gb,
+                        int exp_cols, int transpose) {
+  const int rb = blockIdx.x / n_gb, gb = blockIdx.x % n_gb, t = threadIdx.x;
+  const long long tile = static_cast<long long>(rb) * 4 + (t & 3), r = tile * 32 + (t >> 2);
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int g = gb * 4 + j;
+    uint32_t e = 127;
+    if (r < op_rows && g < op_groups) e = transpose ? tile_exp[static_cast<long long>(g) * exp_cols + tile] : tile_exp[tile * exp_cols + g];
+    word |= e << (8 * j);
+  }
+  reinterpret_cast<uint32_t*>(out)[static_cast<long long>(blockIdx.x) * 128 + t] = word;
 }
 
 // ------------------------------------------------------------------ activation quantiser (1x32 groups)
@@ -733,11 +737,13 @@ FSB_API int fsb_mx_expand_scales(const void* tile_exp, void* out, int rows, int 
   if (rows <= 0 || cols <= 0) return FSB_OK;
   const int op_rows = transpose ? cols : rows;
   const int op_groups = ((transpose ? rows : cols) + 31) / 32;
-  const int pad_rows = (op_rows + 127) / 128 * 128, pad_groups = (op_groups + 3) / 4 * 4;
-  const long long total = static_cast<long long>(pad_rows) * pad_groups;
-  mx_expand_scales_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, stream>>>(
-      static_cast<const uint8_t*>(tile_exp), static_cast<uint8_t*>(out), op_rows, op_groups, pad_rows, pad_groups,
-      (cols + 31) / 32, transpose);
+  if (reinterpret_cast<uintptr_t>(out) & 3) return FSB_ERR_BAD_ARG;
+  const int n_gb = (op_groups + 3) / 4;
+  const long long blocks = (static_cast<long long>(op_rows) + 127) / 128 * n_gb;
+  if (blocks > 0x7fffffffll) return FSB_ERR_TOO_LARGE;
+  mx_expand_scales_kernel<<<static_cast<unsigned>(blocks), 128, 0, stream>>>(static_cast<const uint8_t*>(tile_exp),
+                                                                             static_cast<uint8_t*>(out), op_rows, op_groups, n_gb,
+                                                                             (cols + 31) / 32, transpose);
   return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH;
 }
 

@@ -208,3 +208,10 @@ def test_layer_trains_and_scores_in_a_captured_graph():
     with torch.no_grad():
         assert torch.equal(z, layer(fresh))
     ops.check_status()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (33, 96), (128, 128), (300, 4128), (4100, 160)])
+def test_expanded_tile_exponents_match_the_restatement(rows, cols):
+    e = torch.randint(0, 255, (-(-rows // 32), cols // 32), dtype=torch.uint8)
+    for transpose in (False, True):
+        assert torch.equal(m8.mx_expand_scales(e.cuda(), rows, cols, transpose).cpu(), m8.mx_expand_scales(e, rows, cols, transpose))
