@@ -57,8 +57,12 @@ def _check_operand(q: torch.Tensor, scales: torch.Tensor, what: str) -> None:
     if len(shape) != 2 or q.dtype is not torch.uint8 or shape[1] % (GROUP // 2) or shape[1] == 0:
         raise ValueError(f"{what}: codes must be a uint8 matrix [rows, cols / 2] with cols a multiple of {GROUP}, got "
                          f"{q.dtype}{tuple(shape)}")
-    need = (-(-shape[0] // 128) * 128) * (-(-shape[1] // 64) * 4)        # blocked_scale_numel(rows, cols)
-    if scales.dtype is not torch.uint8 or scales.numel() < need or not scales.is_contiguous() or scales.device != q.device:
+    _check_scales(scales, shape[0], 2 * shape[1], q.device, what)
+
+
+def _check_scales(scales: torch.Tensor, rows: int, cols: int, device, what: str) -> None:
+    need = (-(-rows // 128) * 128) * (-(-cols // 128) * 4)               # blocked_scale_numel(rows, cols)
+    if scales.dtype is not torch.uint8 or scales.numel() < need or not scales.is_contiguous() or scales.device != device:
         raise ValueError(f"{what}: scales must be at least {need} contiguous uint8 bytes in block layout on the codes' device")
 
 
@@ -342,6 +346,7 @@ def mxfp4_linear(x, weight, wq, fwd_scale, dgrad_scale):
                 raise ValueError(f"the input gradient of mxfp4_linear needs dims that are multiples of 128, got {N} x {K}")
             if dgrad_scale is None:
                 raise ValueError("the input gradient of mxfp4_linear needs the scales of the transposed weight (dgrad_scale)")
+            _check_scales(dgrad_scale, K, N, wq.device, "mxfp4_linear (dgrad_scale)")
         if needs_w and (N % 8 or K % 8):
             raise ValueError(f"the weight gradient of mxfp4_linear needs dims that are multiples of 8, got {N} x {K}")
     return _Mxfp4Linear.apply(x, weight, wq, fwd_scale, dgrad_scale)

@@ -189,3 +189,12 @@ def test_refusals():
         w = torch.zeros(36, 128).bfloat16()
         w4 = BlockwiseMxfp4Weight.from_float(w)
         m4.mxfp4_linear(x, w.requires_grad_(), w4.qdata, w4.scale, w4.dgrad_scale)
+
+
+@pytest.mark.parametrize("change", [lambda s: s[:-1], lambda s: s.repeat_interleave(2)[::2], lambda s: s.int(), lambda s: s.to("meta")])
+def test_input_gradient_scales_are_checked(change):
+    """Short, strided, wrongly typed or elsewhere: the products read them by their sizes alone."""
+    x, w4 = torch.zeros(4, 128).bfloat16(), BlockwiseMxfp4Weight.from_float(torch.zeros(256, 128).bfloat16())
+    with pytest.raises(ValueError, match="dgrad_scale.*contiguous uint8"):
+        m4.mxfp4_linear(x.clone().requires_grad_(), None, w4.qdata, w4.scale, change(w4.dgrad_scale))
+    assert m4.mxfp4_linear(x, None, w4.qdata, w4.scale, None).shape == (4, 256)
