@@ -38,6 +38,8 @@ def _ensure():
         _lib.declare("fsb_mx4_quant_weight", [vp, vp, vp, vp, vp, i32, i32, i64, vp])
         _lib.declare("fsb_mx4_expand", [vp, vp, vp, i64, i32, i64, i32, vp])
         _lib.declare("fsb_mxfp4_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i32, vp, vp])
+        _lib.declare("fsb_mxfp4_linear_dx", [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, vp, vp])
+        _lib.declare("fsb_mxfp4_linear_dw", [vp, i64, vp, i64, vp, i32, vp, i32, i32, i32, vp, vp])
         _lib.declare("fsb_gemm_mxfp4", [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, vp, vp])
         _declared = True
 
@@ -277,6 +279,46 @@ def _product_with(x2, wq, fwd_scale):
     return out
 
 
+def _input_gradient(dy2, wq, dgrad_scale):
+    """``dy2 [T, N]`` in MXFP8 groups along N times the codes' own values."""
+    (T, N), K = dy2.shape, 2 * wq.shape[1]
+    if not dy2.is_cuda:
+        return gemm_mxfp8(*mx_quantize_act(dy2), mx4_to_e4m3(wq), dgrad_scale, b_t=True)
+    _ensure()
+    if wq.stride(1) != 1 or wq.stride(0) % 4 or wq.data_ptr() % 4:
+        wq = wq.clone(memory_format=torch.contiguous_format)
+    if dgrad_scale.data_ptr() % 16:
+        dgrad_scale = dgrad_scale.clone()
+    dx = dy2.new_empty(T, K)
+    scratch = torch.empty(T * N + N * K + blocked_scale_numel(T, N), dtype=torch.uint8, device=dy2.device)
+    with _lib.device_of(dy2):
+        rc = _lib.load().fsb_mxfp4_linear_dx(dy2.data_ptr(), N, wq.data_ptr(), wq.stride(0), dgrad_scale.data_ptr(), dx.data_ptr(),
+                                             scratch.data_ptr(), T, N, K, _lib.status_word(dy2.device).data_ptr(),
+                                             _lib.stream_ptr(dy2.device))
+    _lib.check(rc, "fsb_mxfp4_linear_dx")
+    count_launch(3)
+    return dx
+
+
+def _weight_gradient(dy2, x2, dtype):
+    """``dy2^T x2`` with both operands in MXFP8 groups along the rows (all dims multiples of 128)."""
+    (T, N), K = dy2.shape, x2.shape[1]
+    if not dy2.is_cuda:
+        return gemm_mxfp8(*mx_quantize_rows(dy2), *mx_quantize_rows(x2), a_t=True, b_t=True, out_dtype=dtype)
+    _ensure()
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    dw = torch.empty(N, K, dtype=dtype, device=dy2.device)
+    scratch = torch.empty((T + T // 32) * (N + K), dtype=torch.uint8, device=dy2.device)
+    with _lib.device_of(dy2):
+        rc = _lib.load().fsb_mxfp4_linear_dw(dy2.data_ptr(), N, x2.data_ptr(), x2.stride(0), dw.data_ptr(), int(dtype == torch.float32),
+                                             scratch.data_ptr(), T, N, K, _lib.status_word(dy2.device).data_ptr(),
+                                             _lib.stream_ptr(dy2.device))
+    _lib.check(rc, "fsb_mxfp4_linear_dw")
+    count_launch(3)
+    return dw
+
+
 class _Mxfp4Linear(torch.autograd.Function):
     """y = x W^T in 4 bits; gradients in 8 bits with the 4-bit weights' own values (quantisation counts as the identity)."""
 
@@ -301,8 +343,7 @@ class _Mxfp4Linear(torch.autograd.Function):
             if T == 0:
                 dx = torch.zeros(ctx.xshape, dtype=x2.dtype, device=x2.device)
             else:
-                dyq, sdy = mx_quantize_act(dy2)
-                dx = gemm_mxfp8(dyq, sdy, mx4_to_e4m3(wq), dgrad_scale, b_t=True).view(ctx.xshape)
+                dx = _input_gradient(dy2, wq, dgrad_scale).view(ctx.xshape)
         if ctx.needs_input_grad[1]:
             main = getattr(weight, "main_grad", None)
             gd = getattr(weight, "grad_dtype", None) or torch.bfloat16
@@ -314,10 +355,7 @@ class _Mxfp4Linear(torch.autograd.Function):
             elif T == 0:
                 dw = torch.zeros(N, K, dtype=gd, device=x2.device)
             elif MX_WGRAD and T % 128 == 0 and N % 128 == 0 and K % 128 == 0:
-                # contraction over the tokens: both operands in 32x1 groups, read transposed by the tensor core
-                dq, sd = mx_quantize_rows(dy2)
-                xq, sx = mx_quantize_rows(x2)
-                dw = gemm_mxfp8(dq, sd, xq, sx, a_t=True, b_t=True, out_dtype=gd)
+                dw = _weight_gradient(dy2, x2, gd)
             else:
                 dw = gemm(dy2, x2, a_t=True, b_t=True, out_dtype=gd)
         return dx, dw, None, None, None

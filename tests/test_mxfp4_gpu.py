@@ -215,3 +215,35 @@ def test_expanded_tile_exponents_match_the_restatement(rows, cols):
     e = torch.randint(0, 255, (-(-rows // 32), cols // 32), dtype=torch.uint8)
     for transpose in (False, True):
         assert torch.equal(m8.mx_expand_scales(e.cuda(), rows, cols, transpose).cpu(), m8.mx_expand_scales(e, rows, cols, transpose))
+
+
+@pytest.mark.parametrize("T", [1, 5, 127, 128, 384])
+@pytest.mark.parametrize("layout", ["plain", "strided codes", "codes off a word", "scales off a vector", "strided input"])
+def test_gradients_are_those_of_the_separate_operators(T, layout):
+    """The joint entries against the public quantisers and products that they run, bit for bit."""
+    from flex_shard_b200.ops.mxfp8 import gemm_mxfp8, mx_quantize_act, mx_quantize_rows
+
+    N, K = 256, 384
+    g = torch.Generator("cuda").manual_seed(T)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()  # noqa: E731
+    x, w, dy = rand(T, K), rand(N, K), rand(T, N)
+    w4 = BlockwiseMxfp4Weight.from_float(w)
+    wq, sd = w4.qdata, w4.dgrad_scale
+    if layout == "strided codes":
+        wq = torch.cat([wq, wq], 1)[:, : K // 2]
+    elif layout == "codes off a word":
+        wq = torch.cat([wq.flatten()[:1], wq.flatten()])[1:].view(N, K // 2)
+    elif layout == "scales off a vector":
+        sd = torch.cat([sd[:1], sd])[1:]
+    elif layout == "strided input":
+        x = torch.cat([x, x], 1)[:, :K]
+    xg, wg = x.detach().requires_grad_(), w.requires_grad_()
+    for dtype in (torch.bfloat16, torch.float32):
+        wg.grad_dtype = dtype
+        y = m4.mxfp4_linear(xg, wg, wq, w4.scale, sd)
+        dx, dw = torch.autograd.grad(y, (xg, wg), dy)
+        want = gemm_mxfp8(*mx_quantize_act(dy), m4.mx4_to_e4m3(w4.qdata), w4.dgrad_scale, b_t=True)
+        assert torch.equal(dx, want)
+        if T % 128 == 0:
+            want = gemm_mxfp8(*mx_quantize_rows(dy), *mx_quantize_rows(x), a_t=True, b_t=True, out_dtype=dtype)
+            assert dw.dtype == dtype and torch.equal(dw, want)
