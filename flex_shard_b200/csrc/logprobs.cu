@@ -3,7 +3,9 @@
 // With z = x / temperature, m = max z, s = sum e^(z - m), u = sum (z - m) e^(z - m):
 //   log p_j = (z_j - m) - log s,   H = log s - u / s,
 //   dH / dz_j = -p_j (log p_j + H),   d log p_i / dz_j = [i = j] - p_j.
-// z - m is taken as (x - max x) / temperature: differences of logits of the type's lowest value do not overflow.
+// z - m is (x - max x) / temperature wherever it is taken of single logits: differences of logits of the type's lowest value do
+// not overflow, and no error grows with what all logits of a row share. The sums of the forward pass save the subtraction: they
+// are taken relative to m rounded (`Sums`), and what the rounding put in is taken out of their logarithm at the end.
 #include "common.cuh"
 #include <type_traits>
 
@@ -164,11 +166,16 @@ __device__ __forceinline__ float block_reduce(float v, float* red, F op) {
   return v;
 }
 
-// Running sums relative to a maximum m, in base 2: s = sum 2^((x - m) c), u = sum (x - m) c 2^((x - m) c), c = log2(e) / temperature.
+// Running sums in base 2 relative to the rounded product o = fl(-m c) of a maximum m, c = log2(e) / temperature:
+// s = sum 2^(x c + o), u = sum (x c + o) 2^(x c + o). An fma takes x c exactly, so that the exponents' errors are relative to
+// themselves; the maximum counts as 2^over, over = m c + o, and not as 1. |over| is half a step of m c at most: 2 up to FAR, beyond which
+// the sums are not used.
+constexpr float FAR = 0x1p26f;
+__device__ __forceinline__ float offset_of(float m, float c) { return __fmul_rn(-m, c); }
 struct Sums {
   float m, s, u;
   __device__ __forceinline__ void raise(float to, float c) {
-    const float d = (m - to) * c, f = ex2(d);
+    const float d = offset_of(to, c) - offset_of(m, c), f = ex2(d);
     u = (u + s * d) * f;
     s *= f;
     m = to;
@@ -363,9 +370,10 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   const bool inside = tgt >= 0 && tgt < V;
   const float xt = part == 0 && tid == 0 && inside ? to_f(r[tgt]) : 0.f;
   const float c = inv_t * L2E;
-  // Sums start at a finite maximum: a row whose maximum is not above it, or overflows when scaled, or whose sum is not a
-  // finite number, is done again at the end, with differences taken before they are scaled.
-  const float floor_ = fmaxf(-1e38f / c, -3e38f);
+  // Sums start at a finite maximum, so that nothing below it (masked tokens, whatever their number) leaves a trace: a row whose
+  // maximum is not above it, or as far on the other side, or whose sum is not a finite number, is done again at the end, with
+  // differences taken before they are scaled.
+  const float floor_ = -FAR / c;
   const RowSpan span = row_span(r, V);
   const int per = (span.nvec + parts - 1) / parts;
   const int first_vec = min(part * per, span.nvec), end_vec = min(first_vec + per, span.nvec);
@@ -377,7 +385,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   auto take = [&](const uint4 (&v)[4]) {
     const float vm = Vec<T>::largest(v);
     if (vm > a.m) a.raise(vm, c);
-    const float mo = -a.m * c;
+    const float mo = offset_of(a.m, c);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float f[L];
@@ -432,7 +440,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     edge = to_f(r[edge_at]);
     tmax = max_nan(tmax, edge);
     if (edge > a.m) a.raise(edge, c);
-    const float d = max_nan(fmaf(edge, c, -a.m * c), -256.f), e = ex2(d);
+    const float d = max_nan(fmaf(edge, c, offset_of(a.m, c)), -256.f), e = ex2(d);
     a.s += e;
     a.u = fmaf(d, e, a.u);
   }
@@ -496,8 +504,11 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
       __syncthreads();
     }
   }
-  float log_s = logf(all.s), H = log_s - all.u * LN2 / all.s;
-  if (!(all.m > floor_ && fabsf(all.m * c) < 1e38f && fabsf(all.s) < INFINITY)) {      // the same in all threads
+  // The maximum counts as 2^over. A row with one token left is exact: its sum is ex2(over) itself, and its mean differs from `over`
+  // by the roundings of a product and a quotient, 2^-23 |over| together, below which a difference is none.
+  const float over = fmaf(all.m, c, offset_of(all.m, c)), gap = all.u / all.s - over;
+  float log_s = logf(all.s / ex2(over)), H = log_s - (fabsf(gap) <= 0x1p-22f * fabsf(over) ? 0.f : gap) * LN2;
+  if (!(all.m > floor_ && all.m * c < FAR && all.s < INFINITY)) {      // the same in all threads
     auto add = [](float p, float q) { return p + q; };
     float mx = -INFINITY;
     for (int i = tid; i < V; i += THREADS) mx = max_nan(mx, to_f(r[i]));
@@ -517,6 +528,8 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     log_s = logf(s);
     H = log_s - u / s;
   }
+  log_s = max_nan(log_s, 0.f);                       // the sum has a term of 1, and no entropy is negative: roundings aside
+  H = max_nan(H, 0.f);
   if (tid == 0) {
     logprob[row] = inside ? (xt - all.m) * inv_t - log_s : __uint_as_float(0x7fc00000u);
     entropy[row] = H;
@@ -558,12 +571,9 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ targe
   if (tgt < 0 || tgt >= V) G += g * __uint_as_float(0x7fc00000u);      // a target outside the vocabulary: NaN
   const float2 st = stats[row];
   const float m = st.x, log_s = st.y, H = entropy[row], c = inv_t * L2E;
-  const float A = -h * LN2 * inv_t, B = -(G + h * H) * inv_t;
-  // scaled maxima that overflow: differences first, as in the forward pass
-  const bool wide = !(fabsf(m * c) < 1e38f);
-  const float mo = -m * c - log_s * L2E;
+  const float A = -h * LN2 * inv_t, B = -(G + h * H) * inv_t, shift = -log_s * L2E;
   auto smooth = [&](float v) {
-    const float l = max_nan(wide ? (v - m) * c - log_s * L2E : fmaf(v, c, mo), -256.f);
+    const float l = max_nan(fmaf(v - m, c, shift), -256.f);
     return ex2(l) * fmaf(l, A, B);
   };
   const RowSpan span = row_span(r, V);

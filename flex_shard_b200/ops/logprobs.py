@@ -177,6 +177,9 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, *, temperature: f
     ``logprob``, ``entropy`` and ``top_logprob`` (the choice of alternatives counts as constant); the backward pass reads the
     logits again, so they must not be overwritten before it (as ``cross_entropy`` does).
 
+    * Errors grow with a logit's distance from the row's largest over the temperature, not with what the row's logits share; log
+      probabilities are at most 0, entropies at least 0, and both exactly 0 where one token is left. On the GPU a row whose
+      largest logit over the temperature is beyond 4.6e7 in magnitude is read four times instead of once.
     * Alternatives are ordered by logit, the lower index first among equals; a NaN counts as the largest.
     * Rows whose target is ``ignore_index`` are not read: 0 for all values, -1 for the indices, no gradient.
     * Any other target outside the vocabulary gives a NaN log probability (entropy and alternatives are unaffected).
