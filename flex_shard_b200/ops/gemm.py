@@ -39,8 +39,10 @@ class PeerBlocked:
 
 
 def _rowmajor(t: torch.Tensor) -> torch.Tensor:
+    """``t`` or a copy whose rows the copy engine can load. ``contiguous`` does not copy a dense view that starts off a 16-byte
+    boundary, nor a single row of any stride."""
     if t.stride(-1) != 1 or (t.dim() == 2 and t.stride(0) % 8 != 0) or t.data_ptr() % 16 != 0:
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 

@@ -1,0 +1,20 @@
+"""Dense operands that start anywhere in memory: what the host makes of them before a launch."""
+import pytest
+import torch
+
+from flex_shard_b200.ops.gemm import _rowmajor
+
+
+@pytest.mark.parametrize("offset", [0, 1, 4, 7, 8])
+def test_rows_for_the_copy_engine_start_on_a_boundary(offset):
+    base = torch.randn(offset + 16 * 24).bfloat16()
+    x = base[offset:].view(16, 24)
+    y = _rowmajor(x)
+    assert y.data_ptr() % 16 == 0 and y.stride() == (24, 1) and torch.equal(x, y)
+    assert (y.data_ptr() == x.data_ptr()) == (x.data_ptr() % 16 == 0)      # copied only where it has to be
+
+
+def test_a_single_row_of_any_stride():
+    x = torch.randn(64).bfloat16().as_strided((1, 24), (7, 1))              # counts as contiguous
+    y = _rowmajor(x)
+    assert y.stride(0) % 8 == 0 and torch.equal(x, y)
