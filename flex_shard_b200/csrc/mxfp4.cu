@@ -1190,7 +1190,7 @@ FSB_API int fsb_mxfp4_linear(const void* x, long long ldx, const void* bq, long 
   return rc == FSB_OK ? product(q, sf, bq, sfb, a, K / 2, ldb, true, stream) : rc;
 }
 
-// dx[T, K] = Q8(dy) W for dy [T, N] bf16 (row stride lddy, a multiple of 4) and the codes wq [N, K / 2] with the scales of the
+// dx[T, K] = Q8(dy) W for dy [T, N] bf16 (row stride lddy) and the codes wq [N, K / 2] with the scales of the
 // operand [K, N]; N and K multiples of 128. dy in MXFP8 groups along N, the codes as e4m3 with their own scales.
 // scratch: T * N + N * K + pad128(T) * (N / 32) bytes on a 16-byte boundary. One entry for the three launches: the time of a
 // small backward pass is the host's (T = 500, N = K = 2048: forward and both gradients 167.5 us with an entry each, 145.9 so).

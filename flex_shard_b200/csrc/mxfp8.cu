@@ -133,6 +133,10 @@ mx_expand_scales_kernel(const uint8_t* __restrict__ tile_exp, uint8_t* __restric
 
 // ------------------------------------------------------------------ activation quantiser (1x32 groups)
 // Four threads per (row, 32-column group), 8 columns each, two rows' worth of units per thread in flight: bound by memory.
+// vec: every row starts on a 16-byte boundary and its codes on one of 8; otherwise both on half of that, or (ANY) the rows
+// anywhere: a kernel of its own, since a third branch costs the others 1.6 % (8192 x 14336: 76.5 / 75.3 us; a kernel for each of
+// the three 79.5).
+template <bool ANY>
 __global__ void __launch_bounds__(256)
 mx_quant_act_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scales, long long T,
                     int K, long long ldx, long long ldq, int n_gb, int vec) {
@@ -152,10 +156,15 @@ mx_quant_act_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q
     row[j] = live[j] ? i / units : 0;
     u[j] = live[j] ? static_cast<int>(i - row[j] * units) : 0;
     const __nv_bfloat16* p = x + row[j] * ldx + u[j] * 8;
-    if (vec) v[j] = *reinterpret_cast<const uint4*>(p);
-    else {
+    if (!ANY && vec) {
+      v[j] = *reinterpret_cast<const uint4*>(p);
+    } else if (!ANY) {
       const uint2 a = reinterpret_cast<const uint2*>(p)[0], b = reinterpret_cast<const uint2*>(p)[1];
       v[j] = make_uint4(a.x, a.y, b.x, b.y);
+    } else {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+      v[j] = make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
+                        h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
     }
   }
   const unsigned group = 0xfu << (threadIdx.x & 28);
@@ -169,8 +178,9 @@ mx_quant_act_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q
     if ((u[j] & 3) == 0) scales[blocked_offset(row[j], u[j] >> 2, n_gb)] = static_cast<uint8_t>(e);
     const uint2 o = quant8(v[j], e8m0_inv(e));
     uint8_t* d = q + row[j] * ldq + u[j] * 8;
-    if (vec) *reinterpret_cast<uint2*>(d) = o;
-    else {
+    if (!ANY && vec) {
+      *reinterpret_cast<uint2*>(d) = o;
+    } else {
       reinterpret_cast<uint32_t*>(d)[0] = o.x;
       reinterpret_cast<uint32_t*>(d)[1] = o.y;
     }
@@ -747,17 +757,19 @@ FSB_API int fsb_mx_expand_scales(const void* tile_exp, void* out, int rows, int 
   return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH;
 }
 
-// x: bf16 [T, K], K % 128 == 0; q: e4m3 [T, K]; scales: blocked, pad128(T) * (K/32) bytes (rows past T
-// are not written: allocate zeroed or ignore them, they only feed output rows that are masked).
+// x: bf16 [T, K], K % 128 == 0, from any address and with any row stride; q: e4m3 [T, K], its rows on 4-byte boundaries; scales:
+// blocked, pad128(T) * (K/32) bytes (rows past T are not written: allocate zeroed or ignore them, they only feed output rows
+// that are masked).
 FSB_API int fsb_mx_quant_act(const void* x, void* q, void* scales, long long T, int K, long long ldx, long long ldq,
                              cudaStream_t stream) {
-  if (K % 128 != 0 || ldx % 4 != 0 || ldq % 4 != 0) return FSB_ERR_BAD_ARG;
+  if (K % 128 != 0 || ldq % 4 != 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0) return FSB_ERR_BAD_ARG;
   if (T <= 0) return FSB_OK;
   const long long half = (T * (K / 32) + 1) / 2 * 4;   // as in the kernel: threads, two units each
   const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldx % 8 == 0 && ldq % 8 == 0;
-  mx_quant_act_kernel<<<static_cast<unsigned>((half + 255) / 256), 256, 0, stream>>>(
-      static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales), T, K, ldx, ldq,
-      K / 128, vec);
+  const bool words = (reinterpret_cast<uintptr_t>(x) & 7) == 0 && ldx % 4 == 0;
+  auto kernel = vec || words ? mx_quant_act_kernel<false> : mx_quant_act_kernel<true>;
+  kernel<<<static_cast<unsigned>((half + 255) / 256), 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q),
+                                                                        static_cast<uint8_t*>(scales), T, K, ldx, ldq, K / 128, vec);
   return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH;
 }
 

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from flex_shard_b200.ops import _lib
 from flex_shard_b200.ops.gemm import _rowmajor
 
 
@@ -18,3 +19,13 @@ def test_a_single_row_of_any_stride():
     x = torch.randn(64).bfloat16().as_strided((1, 24), (7, 1))              # counts as contiguous
     y = _rowmajor(x)
     assert y.stride(0) % 8 == 0 and torch.equal(x, y)
+
+
+@pytest.mark.skipif(not _lib.lib_path().exists(), reason="the native library is not built")
+@pytest.mark.parametrize("codes,ld", [(4096 + 1, 128), (4096 + 2, 128), (4096, 130)])
+def test_codes_off_a_word_are_refused(codes, ld):
+    """The entry's own check, before anything is launched (the addresses are never used)."""
+    from flex_shard_b200.ops import mxfp8
+
+    mxfp8._ensure()
+    assert _lib.load().fsb_mx_quant_act(8192, codes, 16384, 1, 128, 128, ld, None) == 1

@@ -3,7 +3,9 @@ import pytest
 import torch
 
 from flex_shard_b200 import ops
+from flex_shard_b200.ops import mxfp4, mxfp8
 from flex_shard_b200.ops.gemm import linear
+from flex_shard_b200.quant import BlockwiseMxfp4Weight
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +34,47 @@ def test_bf16_linear(offset):
     got = run(off(x, offset), off(w, offset), off(dy, offset))
     ops.check_status()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("T,K", [(1, 128), (7, 256), (129, 384)])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (2, 0), (4, 0), (6, 0), (0, 1), (3, 2), (0, 4), (4, 4), (8, 8), (1, 7)])
+def test_mxfp8_quantiser(T, K, offset, pad):
+    """Bases and row strides of every alignment."""
+    x = rand(T, K + pad)
+    q, s = mxfp8.mx_quantize_act(off(x, offset)[:, :K])
+    ops.check_status()
+    q_ref, s_ref = mxfp8.mx_quantize_act_ref(x[:, :K].cpu())
+    assert torch.equal(q.cpu().view(torch.uint8), q_ref.view(torch.uint8))
+    assert torch.equal(mxfp8.from_blocked(s, T, K // 32).cpu(), mxfp8.from_blocked(s_ref, T, K // 32))
+
+
+@pytest.mark.parametrize("T", [1, 100, 128])
+@pytest.mark.parametrize("offset", [1, 4, 7])
+def test_block_scaled_linears(T, offset):
+    """Inputs and gradients off a boundary; 128 rows take the 8-bit weight gradient, fewer the bf16 one."""
+    x, w, dy = rand(T, 256), rand(384, 256, seed=1), rand(T, 384, seed=2)
+    w4 = BlockwiseMxfp4Weight.from_float(w)
+    q8, e8 = mxfp8.mx_quantize_weight(w)
+    scales = [mxfp8.mx_expand_scales(e8, 384, 256, transpose) for transpose in (False, True)]
+    for f in (lambda x, w: mxfp4.mxfp4_linear(x, w, w4.qdata, w4.scale, w4.dgrad_scale), lambda x, w: mxfp8.mxfp8_linear(x, w, q8, *scales)):
+
+        def run(x, dy):
+            a, b = x.requires_grad_(), w.detach().requires_grad_()
+            y = f(a, b)
+            return y, *torch.autograd.grad(y, (a, b), dy)
+
+        want, got = run(x.clone(), dy), run(off(x, offset), off(dy, offset))
+        ops.check_status()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_gradient_behind_a_concatenation():
+    """A dense gradient that starts one element into its memory, as an ordinary program makes it."""
+    x, w = rand(8, 128).requires_grad_(), rand(128, 128, seed=1)
+    w4 = BlockwiseMxfp4Weight.from_float(w)
+    weight = rand(8 * 128 + 1, seed=2)
+    y = linear(x, torch.nn.Parameter(w4, requires_grad=False))
+    (dx,) = torch.autograd.grad((torch.cat([torch.ones(1, device="cuda").bfloat16(), y.flatten()]) * weight).sum(), x)
+    y = linear(x, torch.nn.Parameter(w4, requires_grad=False))
+    (want,) = torch.autograd.grad(y, x, weight[1:].clone().view(8, 128))
+    assert torch.equal(dx, want)
