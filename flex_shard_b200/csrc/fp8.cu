@@ -21,7 +21,9 @@ using namespace fsb;
 struct alignas(16) bf16x8 { __nv_bfloat162 v[4]; };
 
 // ------------------------------------------------------------------ weight quantiser (128x128 tiles)
-// grid = (ceil(cols/128), ceil(rows/128)); 256 threads; each thread owns 8 columns x 8 rows.
+// grid = (ceil(cols/128), ceil(rows/128)); 256 threads; each thread owns 8 columns x 8 rows. VEC: every row starts on a
+// 16-byte boundary and its codes on one of 8; otherwise element by element.
+template <bool VEC>
 __global__ void __launch_bounds__(256)
 quant_weight_128x128_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __restrict__ q,
                             float* __restrict__ inv_scale, int rows, int cols, long long ldw,
@@ -36,7 +38,7 @@ quant_weight_128x128_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __rest
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = tr + rg * 8 + i;
-    if (r < rows && c0 + 8 <= cols) {
+    if (VEC && r < rows && c0 + 8 <= cols) {
       const bf16x8 t = *reinterpret_cast<const bf16x8*>(w + r * ldw + c0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -72,7 +74,7 @@ quant_weight_128x128_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __rest
                                    fminf(fmaxf(vals[i][j + 1] * scale, -448.f), 448.f));
       *reinterpret_cast<uint16_t*>(o + j) = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
     }
-    if (c0 + 8 <= cols) {
+    if (VEC && c0 + 8 <= cols) {
       *reinterpret_cast<uint2*>(q + r * ldq + c0) = *reinterpret_cast<const uint2*>(o);
     } else {
       for (int j = 0; j < 8 && c0 + j < cols; ++j) q[r * ldq + c0 + j] = o[j];
@@ -83,7 +85,9 @@ quant_weight_128x128_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __rest
 // ------------------------------------------------------------------ activation quantiser (1x128 groups)
 // Eight threads per (row, 128-column group), 16 columns each: a 32-byte read and a 16-byte write per thread, which keeps
 // enough bytes in flight to be bound by memory (3 bytes an element; a warp per group, 8 bytes a thread, ran at 2.2 TB/s).
-// inv_scale is written [K/128, T] (k-block major).
+// inv_scale is written [K/128, T] (k-block major). vec: every row starts on a 16-byte boundary, and so do its codes; otherwise the
+// rows start on half of that and the codes on words, or (ANY) the rows anywhere.
+template <bool ANY>
 __global__ void __launch_bounds__(256)
 quant_act_1x128_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ inv_scale,
                        long long T, int K, long long ldx, long long ldq, int vec) {
@@ -94,7 +98,10 @@ quant_act_1x128_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict_
   if (row >= T) return;                           // all eight threads of a group leave together
   const __nv_bfloat16* p = x + row * ldx + u * 16;
   alignas(16) __nv_bfloat162 raw[8];
-  if (vec) {
+  if (ANY) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) raw[j] = __halves2bfloat162(p[2 * j], p[2 * j + 1]);
+  } else if (vec) {
     reinterpret_cast<uint4*>(raw)[0] = reinterpret_cast<const uint4*>(p)[0];
     reinterpret_cast<uint4*>(raw)[1] = reinterpret_cast<const uint4*>(p)[1];
   } else {
@@ -118,7 +125,7 @@ quant_act_1x128_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict_
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = __nv_cvt_float2_to_fp8x2(make_float2(f[j].x * scale, f[j].y * scale), __NV_SATFINITE, __NV_E4M3);
   uint8_t* d = q + row * ldq + u * 16;
-  if (vec) {
+  if (!ANY && vec) {
     *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(o);
   } else {
 #pragma unroll
@@ -364,26 +371,30 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 int g_sms[64] = {0};
 }  // namespace
 
-// w: bf16 [rows, cols] (row stride ldw); q: e4m3 bytes [rows, cols] (row stride ldq);
+// w: bf16 [rows, cols] (row stride ldw); q: e4m3 bytes [rows, cols] (row stride ldq), both from any address;
 // inv_scale: fp32 [ceil(rows/128), ceil(cols/128)].
 FSB_API int fsb_fp8_quant_weight(const void* w, void* q, float* inv_scale, int rows, int cols, long long ldw,
                                  long long ldq, cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return FSB_OK;
   dim3 grid((cols + 127) / 128, (rows + 127) / 128);
-  quant_weight_128x128_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(w),
-                                                        static_cast<uint8_t*>(q), inv_scale, rows, cols, ldw,
-                                                        ldq, (cols + 127) / 128);
+  const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldw % 8 == 0 && ldq % 8 == 0;
+  auto kernel = vec ? quant_weight_128x128_kernel<true> : quant_weight_128x128_kernel<false>;
+  kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(w), static_cast<uint8_t*>(q), inv_scale, rows, cols, ldw, ldq,
+                                   (cols + 127) / 128);
   return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH;
 }
 
-// x: bf16 [T, K] with K % 128 == 0; q: e4m3 [T, K]; inv_scale: fp32 [K/128, T].
+// x: bf16 [T, K] with K % 128 == 0, from any address and with any row stride; q: e4m3 [T, K], its rows on 4-byte boundaries;
+// inv_scale: fp32 [K/128, T].
 FSB_API int fsb_fp8_quant_act(const void* x, void* q, float* inv_scale, long long T, int K, long long ldx,
                               long long ldq, cudaStream_t stream) {
-  if (K % 128 != 0 || ldx % 4 != 0 || ldq % 4 != 0) return FSB_ERR_BAD_ARG;
+  if (K % 128 != 0 || ldq % 4 != 0 || (reinterpret_cast<uintptr_t>(q) & 3) != 0) return FSB_ERR_BAD_ARG;
   if (T <= 0) return FSB_OK;
   const long long blocks = (T * (K / 16) + 255) / 256;
   const int vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15) == 0 && ldx % 8 == 0 && ldq % 16 == 0;
-  quant_act_1x128_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+  const bool words = (reinterpret_cast<uintptr_t>(x) & 7) == 0 && ldx % 4 == 0;
+  auto kernel = vec || words ? quant_act_1x128_kernel<false> : quant_act_1x128_kernel<true>;
+  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
       static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(q), inv_scale, T, K, ldx, ldq, vec);
   return cudaGetLastError() == cudaSuccess ? FSB_OK : FSB_ERR_LAUNCH;
 }

@@ -29,3 +29,12 @@ def test_codes_off_a_word_are_refused(codes, ld):
 
     mxfp8._ensure()
     assert _lib.load().fsb_mx_quant_act(8192, codes, 16384, 1, 128, 128, ld, None) == 1
+
+
+@pytest.mark.skipif(not _lib.lib_path().exists(), reason="the native library is not built")
+@pytest.mark.parametrize("codes,ld", [(4096 + 1, 128), (4096 + 2, 128), (4096, 130)])
+def test_fp8_codes_off_a_word_are_refused(codes, ld):
+    from flex_shard_b200.ops import fp8
+
+    fp8._ensure()
+    assert _lib.load().fsb_fp8_quant_act(8192, codes, 16384, 1, 128, 128, ld, None) == 1

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from flex_shard_b200 import ops
-from flex_shard_b200.ops import mxfp4, mxfp8
+from flex_shard_b200.ops import fp8, mxfp4, mxfp8
 from flex_shard_b200.ops.gemm import linear
 from flex_shard_b200.quant import BlockwiseMxfp4Weight
 
@@ -78,3 +78,33 @@ def test_a_gradient_behind_a_concatenation():
     y = linear(x, torch.nn.Parameter(w4, requires_grad=False))
     (want,) = torch.autograd.grad(y, x, weight[1:].clone().view(8, 128))
     assert torch.equal(dx, want)
+
+
+@pytest.mark.parametrize("T,K", [(1, 128), (7, 256), (129, 384)])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (2, 0), (4, 0), (6, 0), (0, 1), (3, 2), (0, 4), (4, 4), (8, 8), (1, 7)])
+def test_fp8_quantisers(T, K, offset, pad):
+    """Bases and row strides of every alignment give the bits of a dense, aligned copy; a weight also with columns that end
+    inside a vector."""
+    x = rand(T, K + pad)
+    got, want = fp8.quantize_act(off(x, offset)[:, :K]), fp8.quantize_act(x[:, :K].clone())
+    ops.check_status()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+    for cols in (K, K - 5):
+        got = fp8.quantize_blockwise(off(x, offset)[:, :cols])
+        q, s = fp8.quantize_blockwise_ref(x[:, :cols].cpu())
+        assert torch.equal(got[0].cpu().view(torch.uint8), q.view(torch.uint8)) and torch.equal(got[1].cpu(), s)
+
+
+@pytest.mark.parametrize("offset", [1, 4, 7])
+def test_fp8_linear(offset):
+    x, w, dy = rand(100, 256), rand(384, 256, seed=1), rand(100, 384, seed=2)
+    q, s = fp8.quantize_blockwise(w)
+
+    def run(x, dy):
+        a, b = x.requires_grad_(), w.detach().requires_grad_()
+        y = fp8.fp8_linear(a, b, q, s)
+        return y, *torch.autograd.grad(y, (a, b), dy)
+
+    want, got = run(x.clone(), dy), run(off(x, offset), off(dy, offset))
+    ops.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
