@@ -45,6 +45,13 @@ constexpr int MAX_CHUNKS = 8;       // chunk maxima a thread keeps
 constexpr int GROUPS = 64;          // groups of threads whose maxima bound the alternatives
 constexpr int CAP = 512;            // candidates a CTA keeps
 constexpr int MAX_PARTS = 8;        // CTAs of a row (a portable cluster)
+// A thread's chunk: 2^chunk_bits(n) of its n vectors, four or more, so that there are MAX_CHUNKS at most (n is 0 in a row too short
+// for a whole vector).
+constexpr int chunk_bits(int n) {
+  int bits = 2;
+  while ((MAX_CHUNKS << bits) < n) ++bits;
+  return bits;
+}
 
 __device__ __forceinline__ float ex2(float v) {
   float r;
@@ -378,7 +385,7 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
   const int per = (span.nvec + parts - 1) / parts;
   const int first_vec = min(part * per, span.nvec), end_vec = min(first_vec + per, span.nvec);
   const int n = (end_vec - first_vec + THREADS - 1) / THREADS;      // vectors of a thread
-  const int cl_bits = max(2, 32 - __clz((n + MAX_CHUNKS - 1) / MAX_CHUNKS - 1));   // a chunk: 2^cl_bits vectors, 4 or more
+  const int cl_bits = TOP ? chunk_bits(n) : 0;
   Sums a{floor_, 0.f, 0.f};
   float tmax = -INFINITY, cmax = -INFINITY;
   int chunk = 0, in_chunk = 0;
