@@ -511,11 +511,9 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
       __syncthreads();
     }
   }
-  // The maximum counts as 2^over. A row with one token left is exact: its sum is ex2(over) itself, and its mean differs from `over`
-  // by the roundings of a product and a quotient, 2^-23 |over| together, below which a difference is none.
-  const float over = fmaf(all.m, c, offset_of(all.m, c)), gap = all.u / all.s - over;
-  float log_s = logf(all.s / ex2(over)), H = log_s - (fabsf(gap) <= 0x1p-22f * fabsf(over) ? 0.f : gap) * LN2;
-  if (!(all.m > floor_ && all.m * c < FAR && all.s < INFINITY)) {      // the same in all threads
+  float log_s = 0.f, H = 0.f;
+  const bool again = !(all.m > floor_ && all.m * c < FAR && all.s < INFINITY);     // the same in all threads
+  if (again) {
     auto add = [](float p, float q) { return p + q; };
     float mx = -INFINITY;
     for (int i = tid; i < V; i += THREADS) mx = max_nan(mx, to_f(r[i]));
@@ -534,6 +532,14 @@ logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, i
     all.m = mx;
     log_s = logf(s);
     H = log_s - u / s;
+  }
+  if (tid >= 32) return;
+  if (!again) {
+    // The maximum counts as 2^over. A row with one token left is exact: its sum is ex2(over) itself, and its mean differs from
+    // `over` by the roundings of a product and a quotient, 2^-23 |over| together, below which a difference is none.
+    const float over = fmaf(all.m, c, offset_of(all.m, c)), gap = all.u / all.s - over;
+    log_s = logf(all.s / ex2(over));
+    H = log_s - (fabsf(gap) <= 0x1p-22f * fabsf(over) ? 0.f : gap) * LN2;
   }
   log_s = max_nan(log_s, 0.f);                       // the sum has a term of 1, and no entropy is negative: roundings aside
   H = max_nan(H, 0.f);
