@@ -2,7 +2,8 @@
 weight's while its payload is quantised data + scales living in a bucket's persistent buffer.
 
 Only ``detach`` / ``alias`` dispatch (what ``nn.Parameter`` construction and autograd bookkeeping
-need); any real math must go through a linear module that understands the payload.
+need), and for ``BlockwiseMxfp4Weight``, which a module keeps, what copies, moves and loads it; any real math must go
+through a linear module that understands the payload.
 Parity: ``blockwise_quant/weight.py:17-110`` of the reference.
 """
 from __future__ import annotations
@@ -126,7 +127,11 @@ class BlockwiseMxfp8Weight(BlockwiseQuantWeight):
 class BlockwiseMxfp4Weight(BlockwiseQuantWeight):
     """MXFP4 weight: packed e2m1 codes ``[out, in / 2]`` with 32x32 tile scales, kept as the tile exponents plus the two
     blocked scale tensors the tensor core reads (``scale``: groups along ``in`` for y = x W^T; ``dgrad_scale``: groups
-    along ``out`` for dx = dy W). Made from a high-precision matrix; ``linear`` and the prequantised layers consume it."""
+    along ``out`` for dx = dy W). Made from a high-precision matrix; ``linear`` and the prequantised layers consume it.
+
+    As a frozen parameter it lasts: ``copy.deepcopy``, ``module.to`` / ``cuda`` / ``cpu`` / ``to_empty`` and ``torch.save`` /
+    ``torch.load`` keep the payload as it is (a dtype is that of the matrix it stands for), and ``load_state_dict`` takes the
+    payload of another frozen weight or quantises a high-precision matrix."""
 
     inner_names = ("qdata", "scale", "dgrad_scale")
 
@@ -151,12 +156,43 @@ class BlockwiseMxfp4Weight(BlockwiseQuantWeight):
                    **meta.get("extra", {}))
 
     def _rebuild(self):
-        return type(self)(self.qdata, self.scale, self.shape, self.dtype, dgrad_scale=self.dgrad_scale, **self.extra)
+        return self._payload_through(lambda t: t, self.dtype)
+
+    def _payload_through(self, fn, dtype) -> "BlockwiseMxfp4Weight":
+        extra = {k: fn(v) if isinstance(v, torch.Tensor) else v for k, v in self.extra.items()}
+        return type(self)(fn(self.qdata), fn(self.scale), self.shape, dtype, dgrad_scale=fn(self.dgrad_scale), **extra)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        aten, kwargs = torch.ops.aten, kwargs or {}
+        if func is aten.copy_.default and isinstance(args[0], cls):
+            return args[0]._take(args[1])
+        if func is aten.clone.default:
+            return args[0]._payload_through(torch.clone, args[0].dtype)
+        dtype = kwargs.get("dtype") or (args[0].dtype if isinstance(args[0], cls) else None)
+        if func in (aten._to_copy.default, aten.empty_like.default) and dtype.is_floating_point:
+            where = {k: kwargs[k] for k in ("device", "non_blocking") if k in kwargs}
+            move = (lambda t: t.to(copy=True, **where)) if func is aten._to_copy.default else (lambda t: torch.empty_like(t, **where))
+            return args[0]._payload_through(move, dtype)
+        return super().__torch_dispatch__(func, types, args, kwargs)
+
+    def _take(self, other: torch.Tensor) -> "BlockwiseMxfp4Weight":
+        if other.shape != self.shape:
+            raise ValueError(f"a matrix {tuple(other.shape)} does not fit the 4-bit weight {tuple(self.shape)}")
+        if not isinstance(other, BlockwiseMxfp4Weight):
+            other = BlockwiseMxfp4Weight.from_float(other.to(self.device))
+        for name in self.inner_names:
+            getattr(self, name).copy_(getattr(other, name))
+        self.extra["tile_exp"].copy_(other.extra["tile_exp"])
+        return self
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         from ..ops.mxfp4 import mx4_dequantize
 
         return mx4_dequantize(self.qdata, self.scale, torch.float32).to(dtype)
+
+
+torch.serialization.add_safe_globals([BlockwiseMxfp4Weight])    # nothing but a container of its payload
 
 
 def blockwise_mxfp8_dequant_weight(fp8_data: torch.Tensor, fwd_scale: torch.Tensor) -> torch.Tensor:
