@@ -164,7 +164,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         if isinstance(weight, BlockwiseMxfp4Weight):
             from .mxfp4 import mxfp4_linear
 
-            return mxfp4_linear(x, None, weight.qdata, weight.scale, weight.dgrad_scale)
+            return mxfp4_linear(x, None, weight.qdata, weight.scale, weight.dgrad_scale, bf16_input_gradient=True)
         if isinstance(weight, BlockwiseMxfp8Weight):
             from .mxfp8 import mxfp8_linear
 

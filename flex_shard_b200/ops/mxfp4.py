@@ -300,6 +300,14 @@ def _input_gradient(dy2, wq, dgrad_scale):
     return dx
 
 
+def _input_gradient_bf16(dy2, wq, fwd_scale):
+    """The same in bf16, for any N and K: the codes' values times their scales are bf16 numbers. N is padded to the product's 8."""
+    w, pad = mx4_dequantize(wq, fwd_scale), -wq.shape[0] % 8
+    if pad:
+        w, dy2 = torch.nn.functional.pad(w, (0, 0, 0, pad)), torch.nn.functional.pad(dy2, (0, pad))
+    return gemm(dy2, w, b_t=True)
+
+
 def _weight_gradient(dy2, x2, dtype):
     """``dy2^T x2`` with both operands in MXFP8 groups along the rows (all dims multiples of 128)."""
     (T, N), K = dy2.shape, x2.shape[1]
@@ -325,7 +333,7 @@ class _Mxfp4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, wq, fwd_scale, dgrad_scale):
         x2 = x.reshape(-1, x.shape[-1])
-        ctx.save_for_backward(x2, wq, dgrad_scale)
+        ctx.save_for_backward(x2, wq, fwd_scale, dgrad_scale)
         ctx.xshape = x.shape
         ctx.weight = weight
         return _product_with(x2, wq, fwd_scale).view(*x.shape[:-1], wq.shape[0])
@@ -333,7 +341,7 @@ class _Mxfp4Linear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x2, wq, dgrad_scale = ctx.saved_tensors
+        x2, wq, fwd_scale, dgrad_scale = ctx.saved_tensors
         weight = ctx.weight
         N, K = wq.shape[0], x2.shape[1]
         dy2 = dy.reshape(-1, N).contiguous()
@@ -342,6 +350,8 @@ class _Mxfp4Linear(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             if T == 0:
                 dx = torch.zeros(ctx.xshape, dtype=x2.dtype, device=x2.device)
+            elif N % 128 or K % 128:
+                dx = _input_gradient_bf16(dy2, wq, fwd_scale).view(ctx.xshape)
             else:
                 dx = _input_gradient(dy2, wq, dgrad_scale).view(ctx.xshape)
         if ctx.needs_input_grad[1]:
@@ -361,11 +371,16 @@ class _Mxfp4Linear(torch.autograd.Function):
         return dx, dw, None, None, None
 
 
-def mxfp4_linear(x, weight, wq, fwd_scale, dgrad_scale):
+def mxfp4_linear(x, weight, wq, fwd_scale, dgrad_scale, *, bf16_input_gradient: bool = False):
     """``x @ W.T`` for bf16 ``x [..., K]`` (K a multiple of 32) and a weight given as MXFP4 codes ``wq [N, K / 2]`` with the
     blocked scales of the operands ``[N, K]`` (forward) and ``[K, N]`` (input gradient; may be ``None`` where no gradient
     of ``x`` is asked for). ``weight`` is the logical parameter that receives the weight gradient, or ``None`` for a frozen
-    weight. Gradients run on the 8-bit products and need N and K in multiples of 128 (``x``'s) and of 8 (the weight's)."""
+    weight.
+
+    The gradient of ``x`` is an 8-bit product with the 4-bit weight's own values and needs N and K in multiples of 128; with
+    ``bf16_input_gradient`` other sizes take a bf16 product with the same values instead of a refusal (as ``linear`` does for
+    frozen weights). The weight's gradient is an 8-bit product where the number of rows, N and K are multiples of 128 and the
+    parameter has no gradient bucket, else a bf16 one, and needs N and K in multiples of 8."""
     if x.dtype != torch.bfloat16:
         raise ValueError(f"mxfp4_linear takes bf16 inputs, got {x.dtype}")
     _check_operand(wq, fwd_scale, "mxfp4_linear")
@@ -379,7 +394,7 @@ def mxfp4_linear(x, weight, wq, fwd_scale, dgrad_scale):
         y = _product_with(x if x.dim() == 2 else x.reshape(-1, K), wq, fwd_scale)       # nothing to differentiate
         return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
     if needs_x or needs_w:
-        if needs_x:
+        if needs_x and not (bf16_input_gradient and (N % 128 or K % 128)):
             if N % 128 or K % 128:
                 raise ValueError(f"the input gradient of mxfp4_linear needs dims that are multiples of 128, got {N} x {K}")
             if dgrad_scale is None:

@@ -212,13 +212,15 @@ class FlexShardMxfp4BlockwiseLinear(FlexShardPrequantizedLinear):
     def forward(self, x):
         w = self.weight
         q, fwd, dgrad = self.payload(w)
-        return mxfp4_linear(x, None if isinstance(w, BlockwiseMxfp4Weight) else w, q, fwd, dgrad)
+        frozen = isinstance(w, BlockwiseMxfp4Weight)
+        return mxfp4_linear(x, None if frozen else w, q, fwd, dgrad, bf16_input_gradient=frozen)
 
 
 def freeze_mxfp4_weights_(module: nn.Module, patterns) -> nn.Module:
     """Replaces the matrices whose dotted names match one of ``patterns`` (``fnmatch``, as in ``BucketSpec``) by their 4-bit
     payloads, for scoring with a frozen model (a teacher, a reference policy): every ``linear`` on such a weight runs the
-    4-bit product, gradients pass through to its input, the weight takes none. For the decoders of this library, for
+    4-bit product, gradients pass through to its input (an 8-bit product where both sides are multiples of 128, else a bf16
+    one), the weight takes none. Stacks of experts' matrices are refused. For the decoders of this library, for
     instance, ``["layers.*.w*", "head.output"]``. The module must not be sharded; other matrices than those that go through
     ``linear`` (an embedding, a router) must not match."""
     from fnmatch import fnmatchcase
