@@ -503,7 +503,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 }
 
 // ------------------------------------------------------------------ few rows: quantised on the way, split along K
-// Up to 16 rows of bf16 against a weight in one launch. The CTAs of a cluster share a tile of 128 weight rows and divide its
+// Up to 16 rows of bf16 against a weight in one launch, as long as a CTA's share of them is FEW_GROUPS groups or less. The CTAs of a cluster share a tile of 128 weight rows and divide its
 // K; each quantises its own columns of the rows straight into shared memory (the 128-byte swizzle's order: one group is one
 // 16-byte chunk) while the weight streams in, and the partial sums meet in the cluster's shared memory, added in CTA order.
 // Bound by the weight's bytes where there are enough of them, else by the latency of one load, one chain of MMAs and the exchange.
@@ -1012,15 +1012,20 @@ bool raise_smem(Kernel kernel, bool (&raised)[64], int bytes) {
   return raised[dev];
 }
 
-// FSB_ERR_TOO_LARGE: the rows' share of a CTA is more than its threads quantise while the weight arrives, or than fits.
-int launch_few(const void* x, const void* bq, const void* sfb, Args a, long long ldx, long long ldb, cudaStream_t stream) {
-  static bool raised[64] = {false};
-  constexpr int MOST_SMEM = 227 * 1024;
-  if (!raise_smem(linear_mxfp4_few_kernel, raised, MOST_SMEM)) return FSB_ERR_LAUNCH;
+// How the rows are divided where they are few: by their quantisation inside the product, unless a CTA's share of them is more than
+// its threads quantise while the weight arrives, or than fits.
+constexpr int MOST_SMEM = 227 * 1024;
+bool few_rows(Args& a) {
+  if (a.M > F_BN) return false;
   const int tiles = (a.N + BM - 1) / BM, num_kb = (a.K + BK - 1) / BK;
   a.split = k_split(tiles, num_kb, 2, 296);
   a.chunk = (num_kb + a.split - 1) / a.split;
-  if (few_smem(a.chunk) > MOST_SMEM || a.M * a.chunk * 8 > FEW_GROUPS) return FSB_ERR_TOO_LARGE;
+  return few_smem(a.chunk) <= MOST_SMEM && a.M * a.chunk * 8 <= FEW_GROUPS;
+}
+int launch_few(const void* x, const void* bq, const void* sfb, const Args& a, long long ldx, long long ldb, cudaStream_t stream) {
+  static bool raised[64] = {false};
+  if (!raise_smem(linear_mxfp4_few_kernel, raised, MOST_SMEM)) return FSB_ERR_LAUNCH;
+  const int tiles = (a.N + BM - 1) / BM;
   CUtensorMap map_w, map_sfw;
   int rc = codes_map(&map_w, bq, a.N, a.K, ldb, BM);
   if (rc == FSB_OK) rc = scales_map(&map_sfw, sfb, a.N, a.K, 1);
@@ -1171,19 +1176,22 @@ FSB_API int fsb_gemm_mxfp4(const void* aq, const void* sfa, const void* bq, cons
   return product(aq, sfa, bq, sfb, a, lda, ldb, false, stream);
 }
 
-// d[M, N] = Q(x) B^T for bf16 x [M, K] with row stride ldx: the quantiser and the product, in one launch for up to 16 rows.
-// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes on a 16-byte boundary; null: FSB_ERR_TOO_LARGE where it takes two.
+// d[M, N] = Q(x) B^T for bf16 x [M, K] with row stride ldx: the quantiser and the product, in one launch for up to 16 rows of which
+// a CTA has up to FEW_GROUPS groups (16 x 6144 x 4096, not 16 x 28672 x 4096, whose tiles leave no CTAs to divide K).
+// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes on a 16-byte boundary; not used where fsb_mxfp4_linear_few says 1, which is
+// where the call is one launch.
+FSB_API int fsb_mxfp4_linear_few(int M, int N, int K) {
+  Args a{M, N, K};
+  return M > 0 && N > 0 && K > 0 && few_rows(a);
+}
 FSB_API int fsb_mxfp4_linear(const void* x, long long ldx, const void* bq, long long ldb, const void* sfb, void* d, long long ldd,
                              void* scratch, int M, int N, int K, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || ldb % 16 != 0) return FSB_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(sfb) | reinterpret_cast<uintptr_t>(bq)) & 15) return FSB_ERR_BAD_ARG;
-  const Args a{M, N, K, 1, 0, d, ldd, 0, status};
-  if (M <= F_BN) {
-    const int rc = launch_few(x, bq, sfb, a, ldx, ldb, stream);
-    if (rc != FSB_ERR_TOO_LARGE) return rc;
-  }
-  if (scratch == nullptr) return FSB_ERR_TOO_LARGE;
-  if (reinterpret_cast<uintptr_t>(scratch) & 15) return FSB_ERR_BAD_ARG;
+  Args a{M, N, K, 1, 0, d, ldd, 0, status};
+  if (few_rows(a)) return launch_few(x, bq, sfb, a, ldx, ldb, stream);
+  a.split = 1;
+  if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15)) return FSB_ERR_BAD_ARG;
   uint8_t* q = static_cast<uint8_t*>(scratch);
   uint8_t* sf = q + static_cast<long long>(M) * (K / 2);      // K / 2 is a multiple of 16
   const int rc = fsb_mx4_quant_act(x, q, sf, M, K, ldx, stream);

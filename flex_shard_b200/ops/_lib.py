@@ -34,9 +34,6 @@ STATUS_NAMES = {
 }
 
 
-TOO_LARGE = 64      # returned by launchers that have another form for the size
-
-
 class NativeError(RuntimeError):
     pass
 

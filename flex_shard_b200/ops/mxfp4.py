@@ -14,6 +14,7 @@ restatement of the same arithmetic.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd import forward_ad
@@ -38,6 +39,7 @@ def _ensure():
         _lib.declare("fsb_mx4_quant_weight", [vp, vp, vp, vp, vp, i32, i32, i64, vp])
         _lib.declare("fsb_mx4_expand", [vp, vp, vp, i64, i32, i64, i32, vp])
         _lib.declare("fsb_mxfp4_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i32, vp, vp])
+        _lib.declare("fsb_mxfp4_linear_few", [i32, i32, i32])
         _lib.declare("fsb_mxfp4_linear_dx", [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, vp, vp])
         _lib.declare("fsb_mxfp4_linear_dw", [vp, i64, vp, i64, vp, i32, vp, i32, i32, i32, vp, vp])
         _lib.declare("fsb_gemm_mxfp4", [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, vp, vp])
@@ -244,6 +246,12 @@ def gemm_mxfp4(aq, sfa, bq, sfb, *, out_dtype: torch.dtype = torch.bfloat16) -> 
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _one_launch(T: int, N: int, K: int) -> bool:
+    """Whether the linear quantises its rows inside the product and needs no scratch (a rule on the sizes alone)."""
+    return bool(_lib.load().fsb_mxfp4_linear_few(T, N, K))
+
+
 def _product_with(x2, wq, fwd_scale):
     """``[T, K]`` rows times the quantised weight: the forward pass of ``mxfp4_linear``."""
     T, K = x2.shape
@@ -262,20 +270,15 @@ def _product_with(x2, wq, fwd_scale):
         ldw = K // 2
     if fwd_scale.data_ptr() % 16:
         fwd_scale = fwd_scale.clone()
-    linear = _lib.load().fsb_mxfp4_linear
-    status = _lib.status_word(x2.device).data_ptr()
-    rc = _lib.TOO_LARGE
+    scratch = None
+    if T > 16 or not _one_launch(T, N, K):      # codes, scales
+        scratch = torch.empty(T * (K // 2) + blocked_scale_numel(T, K), dtype=torch.uint8, device=x2.device)
     with _lib.device_of(x2):
-        stream = _lib.stream_ptr(x2.device)
-        if T <= 4:      # mostly quantised inside the product, which needs no scratch
-            rc = linear(x2.data_ptr(), ldx, wq.data_ptr(), ldw, fwd_scale.data_ptr(), out.data_ptr(), N, None, T, N, K, status, stream)
-        if rc == _lib.TOO_LARGE:
-            scratch = torch.empty(T * (K // 2) + blocked_scale_numel(T, K), dtype=torch.uint8, device=x2.device)  # codes, scales
-            rc = linear(x2.data_ptr(), ldx, wq.data_ptr(), ldw, fwd_scale.data_ptr(), out.data_ptr(), N, scratch.data_ptr(), T, N, K,
-                        status, stream)
-            count_launch()
+        rc = _lib.load().fsb_mxfp4_linear(x2.data_ptr(), ldx, wq.data_ptr(), ldw, fwd_scale.data_ptr(), out.data_ptr(), N,
+                                          None if scratch is None else scratch.data_ptr(), T, N, K,
+                                          _lib.status_word(x2.device).data_ptr(), _lib.stream_ptr(x2.device))
     _lib.check(rc, "fsb_mxfp4_linear")
-    count_launch()
+    count_launch(1 if scratch is None else 2)
     return out
 
 
