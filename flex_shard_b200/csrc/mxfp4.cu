@@ -968,6 +968,12 @@ int scales_map(CUtensorMap* map, const void* sf, long long rows, int K, int box_
   return fsb_make_tmap_2d_plain(map, sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (rows + 127) / 128, words, words, box_rows, 256);
 }
 
+// Bytes of the blocked scales of an operand [rows, cols]; whether scratch memory can be used and holds what is needed.
+long long scale_bytes(long long rows, int cols) { return (rows + 127) / 128 * 128 * ((cols + 127) / 128 * 4); }
+bool fits(const void* scratch, long long bytes, long long need) {
+  return scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 && bytes >= need;
+}
+
 // CTAs along K for `tiles` tiles: as many as there are places for, each with `least` 256-deep steps or more.
 int k_split(long long tiles, int num_kb, int least, int places) {
   const int most = min(MAX_SPLIT, max(1, num_kb / least)), split = static_cast<int>(max(1ll, min(static_cast<long long>(most), places / tiles)));
@@ -1178,33 +1184,35 @@ FSB_API int fsb_gemm_mxfp4(const void* aq, const void* sfa, const void* bq, cons
 
 // d[M, N] = Q(x) B^T for bf16 x [M, K] with row stride ldx: the quantiser and the product, in one launch for up to 16 rows of which
 // a CTA has up to FEW_GROUPS groups (16 x 6144 x 4096, not 16 x 28672 x 4096, whose tiles leave no CTAs to divide K).
-// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes on a 16-byte boundary; not used where fsb_mxfp4_linear_few says 1, which is
+// scratch: M * (K / 2) + pad128(M) * pad4(K / 32) bytes or more, on a 16-byte boundary; not used where fsb_mxfp4_linear_few says 1, which is
 // where the call is one launch.
 FSB_API int fsb_mxfp4_linear_few(int M, int N, int K) {
   Args a{M, N, K};
   return M > 0 && N > 0 && K > 0 && few_rows(a);
 }
 FSB_API int fsb_mxfp4_linear(const void* x, long long ldx, const void* bq, long long ldb, const void* sfb, void* d, long long ldd,
-                             void* scratch, int M, int N, int K, int* status, cudaStream_t stream) {
+                             void* scratch, long long scratch_bytes, int M, int N, int K, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || ldb % 16 != 0) return FSB_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(sfb) | reinterpret_cast<uintptr_t>(bq)) & 15) return FSB_ERR_BAD_ARG;
   Args a{M, N, K, 1, 0, d, ldd, 0, status};
   if (few_rows(a)) return launch_few(x, bq, sfb, a, ldx, ldb, stream);
   a.split = 1;
-  if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15)) return FSB_ERR_BAD_ARG;
+  const long long codes = static_cast<long long>(M) * (K / 2);      // K / 2 is a multiple of 16
+  if (!fits(scratch, scratch_bytes, codes + scale_bytes(M, K))) return FSB_ERR_BAD_ARG;
   uint8_t* q = static_cast<uint8_t*>(scratch);
-  uint8_t* sf = q + static_cast<long long>(M) * (K / 2);      // K / 2 is a multiple of 16
+  uint8_t* sf = q + codes;
   const int rc = fsb_mx4_quant_act(x, q, sf, M, K, ldx, stream);
   return rc == FSB_OK ? product(q, sf, bq, sfb, a, K / 2, ldb, true, stream) : rc;
 }
 
 // dx[T, K] = Q8(dy) W for dy [T, N] bf16 (row stride lddy) and the codes wq [N, K / 2] with the scales of the
 // operand [K, N]; N and K multiples of 128. dy in MXFP8 groups along N, the codes as e4m3 with their own scales.
-// scratch: T * N + N * K + pad128(T) * (N / 32) bytes on a 16-byte boundary. One entry for the three launches: the time of a
+// scratch: T * N + N * K + pad128(T) * (N / 32) bytes or more, on a 16-byte boundary. One entry for the three launches: the time of a
 // small backward pass is the host's (T = 500, N = K = 2048: forward and both gradients 167.5 us with an entry each, 145.9 so).
 FSB_API int fsb_mxfp4_linear_dx(const void* dy, long long lddy, const void* wq, long long ldw, const void* dgrad_scale, void* dx,
-                                void* scratch, int T, int N, int K, int* status, cudaStream_t stream) {
-  if (T <= 0 || N <= 0 || K <= 0 || N % 128 != 0 || K % 128 != 0 || (reinterpret_cast<uintptr_t>(scratch) & 15)) return FSB_ERR_BAD_ARG;
+                                void* scratch, long long scratch_bytes, int T, int N, int K, int* status, cudaStream_t stream) {
+  if (T <= 0 || N <= 0 || K <= 0 || N % 128 != 0 || K % 128 != 0) return FSB_ERR_BAD_ARG;
+  if (!fits(scratch, scratch_bytes, (static_cast<long long>(T) + K) * N + scale_bytes(T, N))) return FSB_ERR_BAD_ARG;
   uint8_t* q = static_cast<uint8_t*>(scratch);
   uint8_t* w = q + static_cast<long long>(T) * N;
   uint8_t* sf = w + static_cast<long long>(N) * K;             // rows past T stay unset: they scale outputs that are not stored
@@ -1215,11 +1223,11 @@ FSB_API int fsb_mxfp4_linear_dx(const void* dy, long long lddy, const void* wq, 
 }
 
 // dw[N, K] = dy^T x in MXFP8 groups of 32 rows, for dy [T, N] and x [T, K] bf16; T, N and K multiples of 128; bf16 or fp32 dw.
-// scratch: T * (N + K) + (T / 32) * (N + K) bytes on a 16-byte boundary.
+// scratch: T * (N + K) + (T / 32) * (N + K) bytes or more, on a 16-byte boundary.
 FSB_API int fsb_mxfp4_linear_dw(const void* dy, long long lddy, const void* x, long long ldx, void* dw, int dw_fp32, void* scratch,
-                                int T, int N, int K, int* status, cudaStream_t stream) {
-  if (T <= 0 || N <= 0 || K <= 0 || T % 128 != 0 || N % 128 != 0 || K % 128 != 0 || (reinterpret_cast<uintptr_t>(scratch) & 15))
-    return FSB_ERR_BAD_ARG;
+                                long long scratch_bytes, int T, int N, int K, int* status, cudaStream_t stream) {
+  if (T <= 0 || N <= 0 || K <= 0 || T % 128 != 0 || N % 128 != 0 || K % 128 != 0) return FSB_ERR_BAD_ARG;
+  if (!fits(scratch, scratch_bytes, (static_cast<long long>(T) + T / 32) * (static_cast<long long>(N) + K))) return FSB_ERR_BAD_ARG;
   uint8_t* a = static_cast<uint8_t*>(scratch);
   uint8_t* b = a + static_cast<long long>(T) * N;
   uint8_t* sa = b + static_cast<long long>(T) * K;

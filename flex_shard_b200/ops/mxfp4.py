@@ -38,10 +38,10 @@ def _ensure():
         _lib.declare("fsb_mx4_quant_act", [vp, vp, vp, i64, i32, i64, vp])
         _lib.declare("fsb_mx4_quant_weight", [vp, vp, vp, vp, vp, i32, i32, i64, vp])
         _lib.declare("fsb_mx4_expand", [vp, vp, vp, i64, i32, i64, i32, vp])
-        _lib.declare("fsb_mxfp4_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i32, vp, vp])
+        _lib.declare("fsb_mxfp4_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, i32, i32, vp, vp])
         _lib.declare("fsb_mxfp4_linear_few", [i32, i32, i32])
-        _lib.declare("fsb_mxfp4_linear_dx", [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, vp, vp])
-        _lib.declare("fsb_mxfp4_linear_dw", [vp, i64, vp, i64, vp, i32, vp, i32, i32, i32, vp, vp])
+        _lib.declare("fsb_mxfp4_linear_dx", [vp, i64, vp, i64, vp, vp, vp, i64, i32, i32, i32, vp, vp])
+        _lib.declare("fsb_mxfp4_linear_dw", [vp, i64, vp, i64, vp, i32, vp, i64, i32, i32, i32, vp, vp])
         _lib.declare("fsb_gemm_mxfp4", [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, vp, vp])
         _declared = True
 
@@ -270,12 +270,13 @@ def _product_with(x2, wq, fwd_scale):
         ldw = K // 2
     if fwd_scale.data_ptr() % 16:
         fwd_scale = fwd_scale.clone()
-    scratch = None
-    if T > 16 or not _one_launch(T, N, K):      # codes, scales
-        scratch = torch.empty(T * (K // 2) + blocked_scale_numel(T, K), dtype=torch.uint8, device=x2.device)
+    scratch, size = None, 0
+    if T > 16 or not _one_launch(T, N, K):
+        size = T * (K // 2) + blocked_scale_numel(T, K)     # codes, scales
+        scratch = torch.empty(size, dtype=torch.uint8, device=x2.device)
     with _lib.device_of(x2):
         rc = _lib.load().fsb_mxfp4_linear(x2.data_ptr(), ldx, wq.data_ptr(), ldw, fwd_scale.data_ptr(), out.data_ptr(), N,
-                                          None if scratch is None else scratch.data_ptr(), T, N, K,
+                                          None if scratch is None else scratch.data_ptr(), size, T, N, K,
                                           _lib.status_word(x2.device).data_ptr(), _lib.stream_ptr(x2.device))
     _lib.check(rc, "fsb_mxfp4_linear")
     count_launch(1 if scratch is None else 2)
@@ -293,10 +294,11 @@ def _input_gradient(dy2, wq, dgrad_scale):
     if dgrad_scale.data_ptr() % 16:
         dgrad_scale = dgrad_scale.clone()
     dx = dy2.new_empty(T, K)
-    scratch = torch.empty(T * N + N * K + blocked_scale_numel(T, N), dtype=torch.uint8, device=dy2.device)
+    size = T * N + N * K + blocked_scale_numel(T, N)
+    scratch = torch.empty(size, dtype=torch.uint8, device=dy2.device)
     with _lib.device_of(dy2):
         rc = _lib.load().fsb_mxfp4_linear_dx(dy2.data_ptr(), N, wq.data_ptr(), wq.stride(0), dgrad_scale.data_ptr(), dx.data_ptr(),
-                                             scratch.data_ptr(), T, N, K, _lib.status_word(dy2.device).data_ptr(),
+                                             scratch.data_ptr(), size, T, N, K, _lib.status_word(dy2.device).data_ptr(),
                                              _lib.stream_ptr(dy2.device))
     _lib.check(rc, "fsb_mxfp4_linear_dx")
     count_launch(3)
@@ -320,10 +322,11 @@ def _weight_gradient(dy2, x2, dtype):
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
     dw = torch.empty(N, K, dtype=dtype, device=dy2.device)
-    scratch = torch.empty((T + T // 32) * (N + K), dtype=torch.uint8, device=dy2.device)
+    size = (T + T // 32) * (N + K)
+    scratch = torch.empty(size, dtype=torch.uint8, device=dy2.device)
     with _lib.device_of(dy2):
         rc = _lib.load().fsb_mxfp4_linear_dw(dy2.data_ptr(), N, x2.data_ptr(), x2.stride(0), dw.data_ptr(), int(dtype == torch.float32),
-                                             scratch.data_ptr(), T, N, K, _lib.status_word(dy2.device).data_ptr(),
+                                             scratch.data_ptr(), size, T, N, K, _lib.status_word(dy2.device).data_ptr(),
                                              _lib.stream_ptr(dy2.device))
     _lib.check(rc, "fsb_mxfp4_linear_dw")
     count_launch(3)
