@@ -264,7 +264,7 @@ def _product_with(x2, wq, fwd_scale):
     _ensure()
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
-    ldx, ldw = _ld(x2), _ld(wq)
+    ldx, ldw = x2.stride(0) if T > 1 else K, wq.stride(0) if N > 1 else K // 2
     if wq.stride(1) != 1 or ldw % 16 or wq.data_ptr() % 16:
         wq = wq.clone(memory_format=torch.contiguous_format)
         ldw = K // 2
