@@ -223,7 +223,7 @@ class _SwiGLU(torch.autograd.Function):
         F = g2.shape[1] // 2
         dh2 = dh.reshape(-1, F)
         if g2.is_cuda:
-            dh2 = dh2.contiguous()
+            g2, dh2 = g2.contiguous(), dh2.contiguous()
             dgu = torch.empty_like(g2)
             rc = _lib.load().fsb_swiglu_bwd(g2.data_ptr(), dh2.data_ptr(), dgu.data_ptr(), g2.shape[0], F,
                                             _s(g2.device))
