@@ -135,6 +135,12 @@ def device_of(tensor):
     return _same_device if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
+def dense(t):
+    """``t``, or a copy of it, with its elements one after the other from a 16-byte boundary, as kernels read them in vectors.
+    ``contiguous`` does not copy a dense view that starts elsewhere (a gradient behind a concatenation, for instance)."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def plain(*tensors) -> bool:
     """Whether a kernel may be given these tensors' addresses: no subclasses, and no tensors without memory of their own
     (those that ``vmap``, batched gradients and the ``torch.func`` transforms hand to an operator)."""

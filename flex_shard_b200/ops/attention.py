@@ -115,6 +115,7 @@ class _QKVAttention(torch.autograd.Function):
             ctx.dims = (B, S, Hq, Hkv)
             return o.detach().to(qkv.dtype).reshape(B, S, Hq * HD)
         assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous()
+        qkv = _lib.dense(qkv)
         if rope_table is not None:   # query and key heads are neighbours: one launch
             _rope_inplace(qkv[..., : (Hq + Hkv) * HD].view(B, S, Hq + Hkv, HD), rope_table, False)
         o = torch.empty(B, S, Hq * HD, dtype=qkv.dtype, device=qkv.device)
@@ -142,7 +143,7 @@ class _QKVAttention(torch.autograd.Function):
         _ensure()
         qkv, o, lse, rope_table = ctx.saved_tensors
         C = qkv.shape[-1]
-        d_o = d_o.contiguous()
+        d_o = _lib.dense(d_o)
         dev = qkv.device
         dqkv = torch.empty_like(qkv)
         # the fp32 dQ accumulator and, in ordered mode, the turn counters behind it: one zero-fill

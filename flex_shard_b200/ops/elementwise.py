@@ -32,12 +32,12 @@ class _RMSNorm(torch.autograd.Function):
         x2 = x.reshape(-1, D)
         T = x2.shape[0]
         if x.is_cuda:
-            x2 = x2.contiguous()
+            x2 = _lib.dense(x2)
             y = torch.empty_like(x2)
             rstd = torch.empty(T, dtype=torch.float32, device=x.device)
-            w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
+            w = _lib.dense(weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16))
             if residual is not None:
-                r2 = residual.reshape(-1, D).contiguous()
+                r2 = _lib.dense(residual.reshape(-1, D))
                 s = torch.empty_like(x2)
             else:
                 r2, s = None, None
@@ -68,12 +68,12 @@ class _RMSNorm(torch.autograd.Function):
         dy2 = dy.reshape(-1, D)
         dres = dsum.reshape(-1, D) if (ctx.has_res and dsum is not None) else None
         if xin.is_cuda:
-            dy2 = dy2.contiguous()
-            dres = dres.contiguous() if dres is not None else None
+            dy2 = _lib.dense(dy2)
+            dres = _lib.dense(dres) if dres is not None else None
             dx = torch.empty_like(xin)
             nblk = (T + 31) // 32
             partial = torch.empty(nblk, D, dtype=torch.float32, device=xin.device)
-            w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
+            w = _lib.dense(weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16))
             main = getattr(weight, "main_grad", None)
             use_main = main is not None and main.dtype == torch.float32 and main.dim() == 1 and main.is_contiguous()
             if use_main:
@@ -207,7 +207,7 @@ class _SwiGLU(torch.autograd.Function):
         ctx.save_for_backward(g2)
         ctx.shape = gu.shape
         if gu.is_cuda:
-            g2 = g2.contiguous()
+            g2 = _lib.dense(g2)
             h = torch.empty(g2.shape[0], F, dtype=gu.dtype, device=gu.device)
             rc = _lib.load().fsb_swiglu_fwd(g2.data_ptr(), h.data_ptr(), g2.shape[0], F, _s(gu.device))
             _lib.check(rc, "fsb_swiglu_fwd")
@@ -223,7 +223,7 @@ class _SwiGLU(torch.autograd.Function):
         F = g2.shape[1] // 2
         dh2 = dh.reshape(-1, F)
         if g2.is_cuda:
-            g2, dh2 = g2.contiguous(), dh2.contiguous()
+            g2, dh2 = _lib.dense(g2), _lib.dense(dh2)
             dgu = torch.empty_like(g2)
             rc = _lib.load().fsb_swiglu_bwd(g2.data_ptr(), dh2.data_ptr(), dgu.data_ptr(), g2.shape[0], F,
                                             _s(g2.device))

@@ -154,13 +154,13 @@ class _Dispatch(torch.autograd.Function):
     def forward(ctx, x, plan: RoutePlan):
         ctx.plan = plan
         ctx.T = x.shape[0]
-        return _gather(x.contiguous(), plan.src, None, plan.max_rows, x.shape[1])
+        return _gather(_lib.dense(x), plan.src, None, plan.max_rows, x.shape[1])
 
     @staticmethod
     def backward(ctx, dxp):
         plan = ctx.plan
         T, k = plan.pos.shape
-        return _combine(dxp.contiguous(), plan.pos, None, T, k, dxp.shape[1]), None
+        return _combine(_lib.dense(dxp), plan.pos, None, T, k, dxp.shape[1]), None
 
 
 class _Combine(torch.autograd.Function):
@@ -169,7 +169,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w, plan: RoutePlan):
         T, k = plan.pos.shape
-        rows = rows.contiguous()
+        rows = _lib.dense(rows)
         w = w.float().contiguous()
         ctx.save_for_backward(rows, w)
         ctx.plan = plan
@@ -181,7 +181,7 @@ class _Combine(torch.autograd.Function):
         plan = ctx.plan
         T, k = plan.pos.shape
         D = rows.shape[1]
-        dy = dy.contiguous()
+        dy = _lib.dense(dy)
         # row r = (t, k): scale[r] = w[t, k]; rows of padding get index -1
         scale = torch.zeros(plan.max_rows, dtype=torch.float32, device=dy.device)
         scale[plan.pos.reshape(-1).long()] = w.reshape(-1)
@@ -244,7 +244,7 @@ class _GroupedLinear(torch.autograd.Function):
         x, weight = ctx.saved_tensors
         plan = ctx.plan
         E, N, K = weight.shape
-        dy = dy.contiguous()
+        dy = _lib.dense(dy)
         dx = dw = None
         if not x.is_cuda:
             offs = plan.offs.tolist()

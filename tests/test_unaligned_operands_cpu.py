@@ -38,3 +38,12 @@ def test_fp8_codes_off_a_word_are_refused(codes, ld):
 
     fp8._ensure()
     assert _lib.load().fsb_fp8_quant_act(8192, codes, 16384, 1, 128, 128, ld, None) == 1
+
+
+@pytest.mark.parametrize("offset", [0, 1, 8])
+def test_dense(offset):
+    base = torch.randn(offset + 64)
+    x = base[offset:].view(4, 16)
+    y = _lib.dense(x)
+    assert y.data_ptr() % 16 == 0 and torch.equal(x, y) and (y is x) == (x.data_ptr() % 16 == 0)
+    assert _lib.dense(x.t()).is_contiguous() and torch.equal(_lib.dense(x.t()), x.t())

@@ -3,7 +3,10 @@ import pytest
 import torch
 
 from flex_shard_b200 import ops
-from flex_shard_b200.ops import fp8, mxfp4, mxfp8
+from flex_shard_b200.ops import attention
+from flex_shard_b200.ops import elementwise as ew
+from flex_shard_b200.ops import fp8, moe, mxfp4, mxfp8
+from flex_shard_b200.ops.attention import qkv_attention
 from flex_shard_b200.ops.gemm import linear
 from flex_shard_b200.quant import BlockwiseMxfp4Weight
 
@@ -108,3 +111,60 @@ def test_fp8_linear(offset):
     want, got = run(x.clone(), dy), run(off(x, offset), off(dy, offset))
     ops.check_status()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def same(f, inputs, gradients, offset):
+    """Outputs and gradients of ``f`` from aligned inputs and from those that start ``offset`` elements into their memory."""
+    results = []
+    for at in (0, offset):
+        xs = [off(x, at).requires_grad_() for x in inputs]
+        ys = f(*xs)
+        ys = ys if isinstance(ys, tuple) else (ys,)
+        results.append([*ys, *torch.autograd.grad(ys, xs, [off(g, at) for g in gradients])])
+    ops.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("offset", [1, 4])
+def test_norms_and_activation(offset):
+    x, r, w = rand(37, 256), rand(37, 256, seed=1), rand(256, seed=2)
+    same(lambda x, w: ew.rmsnorm(x, w), (x, w), (r,), offset)
+    same(lambda x, r, w: ew.add_rmsnorm(x, r, w), (x, r, w), (rand(37, 256, seed=3), rand(37, 256, seed=4)), offset)
+    same(ew.swiglu, (x,), (rand(37, 128, seed=3),), offset)
+
+
+@pytest.mark.parametrize("offset", [1, 4])
+def test_attention(offset):
+    """The input is rotated in place on the GPU, so every run has its own."""
+    B, S = 1, 128
+    table = ew.rope_table(S, 128, 10000.0, "cuda")
+    o = qkv_attention(off(rand(B, S, 4 * 128), 0), table, 2, 1)
+    p = qkv_attention(off(rand(B, S, 4 * 128), offset), table, 2, 1)
+    assert torch.equal(o, p)
+    attention.set_deterministic(True)           # otherwise the query gradient is added up in any order
+    try:
+        results = []
+        for at in (0, offset):
+            x = rand(B, S, 4 * 128).requires_grad_()
+            y = qkv_attention(x * 1, table, 2, 1)
+            results.append(torch.autograd.grad(y, x, off(rand(B, S, 2 * 128, seed=1), at))[0])
+        ops.check_status()
+    finally:
+        attention.set_deterministic(None)
+    assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("offset", [1, 4])
+def test_experts(offset):
+    T, k, E, D, F = 100, 2, 4, 128, 256
+    plan = moe.plan_routes(torch.stack([torch.randperm(E, device="cuda")[:k] for _ in range(T)]), E)
+    same(lambda x: moe.moe_dispatch(x, plan), (rand(T, D),), (rand(plan.max_rows, D, seed=1),), offset)
+    rows, w = moe.moe_dispatch(rand(T, D), plan), torch.rand(T, k, device="cuda")
+    same(lambda r: moe.moe_combine(r, w, plan), (rows,), (rand(T, D, seed=2),), offset)
+    weight = rand(E, F, D, seed=3)
+    live = (plan.src >= 0)[:, None]
+    x = rows.detach().requires_grad_()
+    dy = rand(plan.max_rows, F, seed=4) * live
+    got = [torch.autograd.grad(moe.grouped_linear(x, weight, plan), x, off(dy, at))[0] * live for at in (0, offset)]
+    ops.check_status()
+    assert torch.equal(*got)
