@@ -159,8 +159,9 @@ class BlockwiseMxfp4Weight(BlockwiseQuantWeight):
         return self._payload_through(lambda t: t, self.dtype)
 
     def _payload_through(self, fn, dtype) -> "BlockwiseMxfp4Weight":
-        extra = {k: fn(v) if isinstance(v, torch.Tensor) else v for k, v in self.extra.items()}
-        return type(self)(fn(self.qdata), fn(self.scale), self.shape, dtype, dgrad_scale=fn(self.dgrad_scale), **extra)
+        each = lambda v: fn(v) if isinstance(v, torch.Tensor) else v  # noqa: E731
+        return type(self)(each(self.qdata), each(self.scale), self.shape, dtype, dgrad_scale=each(self.dgrad_scale),
+                          **{k: each(v) for k, v in self.extra.items()})
 
     @classmethod
     def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
@@ -181,9 +182,13 @@ class BlockwiseMxfp4Weight(BlockwiseQuantWeight):
             raise ValueError(f"a matrix {tuple(other.shape)} does not fit the 4-bit weight {tuple(self.shape)}")
         if not isinstance(other, BlockwiseMxfp4Weight):
             other = BlockwiseMxfp4Weight.from_float(other.to(self.device))
-        for name in self.inner_names:
-            getattr(self, name).copy_(getattr(other, name))
-        self.extra["tile_exp"].copy_(other.extra["tile_exp"])
+        own, theirs = ({**{n: getattr(w, n) for n in self.inner_names}, **w.extra} for w in (self, other))
+        own = {k: v for k, v in own.items() if isinstance(v, torch.Tensor)}
+        if any(theirs.get(k) is None or theirs[k].shape != v.shape for k, v in own.items()):
+            raise ValueError(f"a 4-bit weight that holds {[k for k, v in theirs.items() if v is not None]} cannot be loaded into one "
+                             f"that holds {list(own)}")
+        for k, v in own.items():
+            v.copy_(theirs[k])
         return self
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:

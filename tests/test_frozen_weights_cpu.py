@@ -115,3 +115,16 @@ def test_refusals():
     w = a.head.output.detach()
     with pytest.raises(ValueError, match="does not fit"):
         w.copy_(torch.zeros(1, 128).bfloat16())
+
+
+def test_weights_that_only_score():
+    """Payloads without the input gradient's scales and without tile exponents, as a user may put them together."""
+    full = frozen().head.output.detach()
+    lean = BlockwiseMxfp4Weight(full.qdata.clone(), full.scale.clone(), full.shape)
+    for w in (lean.clone(), lean.to(torch.float32), copy.deepcopy(torch.nn.Parameter(lean, requires_grad=False)), lean.to("meta")):
+        assert w.dgrad_scale is None and w.extra == {} and w.shape == full.shape
+    lean.qdata.zero_()
+    lean.copy_(full)
+    assert torch.equal(lean.qdata, full.qdata)
+    with pytest.raises(ValueError, match="cannot be loaded"):
+        full.copy_(lean)
