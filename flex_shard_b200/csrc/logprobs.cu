@@ -346,7 +346,7 @@ __device__ __forceinline__ void part_top(const T* r, int first_vec, int end_vec,
 // alternatives with the first one). Every thread keeps a running maximum and sums relative to it, and the maxima of its chunks
 // for the alternatives. Bound by memory, closely followed by the issue of instructions (some ten an element at first): the
 // maximum of four vectors at a time and loads without bounds checks but for the row's rest, 8192 x 128256 bf16 343 -> 317 us
-// (6.6 TB/s) without alternatives, 432 -> 389 with 8.
+// (6.6 TB/s) without alternatives, 432 -> 389 with 8 (347 to 390 from one GPU to another).
 template <typename T, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, (sizeof(T) == 4 ? 1536 : 1280) / THREADS)
 logprobs_kernel(const T* __restrict__ x, const long long* __restrict__ target, int V, const Rows rows, float inv_t, int k,
